@@ -353,7 +353,7 @@ def run(state):
     from moondream_amd.beams import reorder_states, select_beams
 
     tokens, parents, scores, ended = select_beams(s["logits"], s["scores"], ended=s["ended"], end_id=END)
-    reorder_states([x for old in s["states"] for x in old], parents, into=[x for new in s["into"] for x in new])
+    reorder_states(s["states"], parents, into=s["into"], slot_dim=1)
     return [tokens, parents, scores, ended, *s["into"]]
 
 

@@ -841,6 +841,138 @@ md_status md_gemm_f32(const void* a, int64_t lda, const md_linear* lin, void* c,
  * attention of any.  Default 3.  Process-wide. */
 void md_lm_set_kernels(int32_t mask);
 
+/* ------------------------------------------------------------------ *
+ * A cache in 8 bits with block scales                                 *
+ * ------------------------------------------------------------------ */
+
+/* One layer's keys and values as OCP e4m3fn numbers, one scale for each block of MD_KV8_BLOCK tokens and head, keys and values apart:
+ *   k, v          codes: row r of head h of a slot at slot * slot_stride + (h * ctx + r) * head_dim bytes
+ *   k_exp, v_exp  bytes, block r / MD_KV8_BLOCK of head h at slot * exp_stride + h * (ctx / MD_KV8_BLOCK) + block:
+ *                 value = code * 2^(byte - 127)
+ * The scale is the least power of two 2^e, MD_KV8_MIN_EXP <= e <= MD_KV8_MAX_EXP, that keeps the block's largest finite magnitude within
+ * 448 * 2^e: an e4m3 number's relative precision does not hang on its scale, and with powers of two a code that moves to another
+ * scale changes only where it becomes subnormal.  What append writes is always a number: NaN counts as 0, what lies beyond 448 * 2^e
+ * (infinities) saturates.
+ * Rows are rows of the cache, in the order of their tokens; a row is not a position once rows have been evicted (keys are cached rotated).
+ * head_dim 64 or 128; ctx % 32 == 0; k, v 16-byte aligned, slot_stride % 16 == 0.
+ * `slot` (device int32 [batch], NULL: sequence b has slot b): a slot outside [0, slots) is an absent sequence: it writes nothing to the
+ * cache, reads as zeros and its outputs are zeros.  A slot may serve several sequences that read it, but one that writes it. */
+#define MD_KV8_BLOCK 32
+#define MD_KV8_MIN_EXP (-40)
+#define MD_KV8_MAX_EXP 40
+typedef struct {
+  void* k;
+  void* v;
+  void* k_exp;
+  void* v_exp;
+  int64_t slot_stride, exp_stride; /* bytes */
+  int32_t slots, ctx, kv_heads, head_dim;
+} md_kv8_cache;
+
+/* Rows row0[b] .. row0[b] + n_new[b] - 1 of every sequence (n_new NULL: q_len) from bf16 keys and values, element (b, t, h, d) at
+ * b * bs + t * ts + h * hs + d, 16-byte aligned, strides % 8 == 0.  Rows past ctx are dropped.  A block that began before row0 keeps at
+ * least its scale; where the new rows need a larger one its older rows are rounded to that.  Other rows stay as they are. */
+md_status md_kv8_append(const md_kv8_cache* cache, const void* k, int64_t k_bs, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_bs,
+                        int64_t v_ts, int64_t v_hs, const int32_t* slot, const int32_t* row0, const int32_t* n_new, int32_t batch,
+                        int32_t q_len, void* stream);
+
+/* Rows row0[b] .. row0[b] + rows - 1 as bf16 (exactly what the codes stand for): k_out, v_out contiguous [batch][kv_heads][rows][head_dim],
+ * 16-byte aligned.  Rows outside [0, min(kv_len[b], ctx)) (kv_len NULL: ctx) read as zeros; row0 NULL: 0. */
+md_status md_kv8_read(const md_kv8_cache* cache, const int32_t* slot, const int32_t* row0, const int32_t* kv_len, int32_t batch, int32_t rows,
+                      void* k_out, void* v_out, void* stream);
+
+/* Softmax attention of q_len queries per sequence over the cache, for single tokens and prompts, any n_heads that kv_heads divides
+ * (query head h reads head h / (n_heads / kv_heads)).  q, o: bf16, element (b, t, h, d) at b * bs + t * ts + h * hs + d, 16-byte aligned,
+ * strides % 8 == 0.  Query t of sequence b stands at row p = q_pos0[b] + t (q_pos0 NULL: the last q_rows[b] rows, kv_len[b] - q_rows[b] + t)
+ * and sees the rows j <= p, with p < prefix_len all j < prefix_len, in every case j < kv_len[b] only; one that sees no row gives zeros.
+ * Queries t >= q_rows[b] (NULL: q_len) are padding: their outputs stay as they are.
+ * max_len bounds kv_len (longer ones count as max_len; 0: ctx) and sizes the launch.
+ * weights (fp32 [slots][kv_heads][ctx], or NULL): weights[row] = decay * weights[row] + the sum over the sequence's queries and the
+ * group's heads of the softmax weight that the row got, for the rows below kv_len; decay 0 does not read what was there.  With
+ * weights a slot may appear once in a call.
+ * Scores, softmax statistics, outputs and weights are held in fp32; a key's softmax weight enters the product with the values as fp16. */
+typedef struct {
+  const void* q;
+  int64_t q_bs, q_ts, q_hs;
+  void* o;
+  int64_t o_bs, o_ts, o_hs;
+  int32_t batch, n_heads, q_len;
+  const int32_t* slot;
+  const int32_t* q_pos0;
+  const int32_t* q_rows;
+  const int32_t* kv_len;
+  int32_t max_len, prefix_len;
+  float scale;
+  float decay;
+  float* weights;
+  void* workspace;
+  size_t workspace_bytes;
+} md_kv8_attn_args;
+size_t md_kv8_attention_workspace_bytes(const md_kv8_cache* cache, const md_kv8_attn_args* args);
+md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_attn_args* args, void* stream);
+
+/* Eviction: of every sequence and head the rows [0, first), the last `recent` ones and those of the largest weights stay, `keep` in all
+ * (all of them while kv_len[b] <= keep); ties: the lower row stays; a NaN weight is the least.  They move together to the rows 0 .. of the
+ * same slot of `to`, in their order, every block with the scale that its rows need now.  `to` is the same cache (in place) or
+ * one that shares no memory with it, of as many heads, the same head_dim and ctx >= keep.
+ * weights: fp32 [slots][kv_heads][ctx] of `from`; weights_out: the same of `to` (NULL: not wanted; in place: weights itself).
+ * kept (int32 [batch][kv_heads][keep]): the rows that stayed, -1 behind the last;  len_out[b] = min(kv_len[b], keep), may be kv_len.
+ * A slot may appear once in a call.  first + recent <= keep. */
+typedef struct {
+  const float* weights;
+  float* weights_out;
+  const int32_t* slot;
+  const int32_t* kv_len;
+  int32_t* len_out;
+  int32_t* kept;
+  int32_t batch, keep, first, recent;
+} md_kv8_evict_args;
+md_status md_kv8_evict(const md_kv8_cache* from, const md_kv8_cache* to, const md_kv8_evict_args* args, void* stream);
+
+/* ------------------------------------------------------------------ *
+ * Beams                                                               *
+ * ------------------------------------------------------------------ */
+
+/* The best continuations of `beams` beams for each of `batch` inputs.  logits: [batch * beams][ld], bf16 or fp32 (dtype MD_DTYPE_*).
+ *   total(k, t) = scores[b][k] + logits[t] - log sum_v exp(logits[v])      of a beam that goes on (logits[suppress_id] = -inf)
+ *   total(k, end_id) = scores[b][k], no other token                        of a beam that has ended (ended[b][k] != 0)
+ * The `beams` largest total * rank_weight[b][k] (fp32, > 0; NULL: 1) are taken, in falling order; ties: the lower beam, then the larger logit,
+ * then the lower token.  A beam whose score is -inf or NaN has no continuations, nor has a total of -inf (how a search begins: all
+ * scores but the first -inf).  Sums and totals are taken in 64 bits.  NaN logits count as -inf, +inf as the largest float.
+ *   tokens, parents [batch][beams]: the token, and the beam (of the same input) that it goes on from
+ *   scores_out: its total;  ended_out: its beam had ended or the token is end_id.  May be scores / ended.
+ * Where fewer continuations are left: token end_id, parent the place itself, score -inf, ended.
+ * ended NULL: none has; end_id -1: no token ends a beam (then ended is NULL).  ended_out may be NULL.  2 <= beams <= MD_MAX_BEAMS. */
+#define MD_MAX_BEAMS 16
+typedef struct {
+  const void* logits;
+  int64_t ld;
+  int32_t dtype, batch, beams, vocab, suppress_id, end_id;
+  const float* scores;
+  const int32_t* ended;
+  const float* rank_weight;
+  int32_t* tokens;
+  int32_t* parents;
+  float* scores_out;
+  int32_t* ended_out;
+  void* workspace;
+  size_t workspace_bytes;
+} md_beam_args;
+size_t md_beam_workspace_bytes(int32_t batch, int32_t beams, int32_t vocab);
+md_status md_beam_select(const md_beam_args* args, void* stream);
+
+/* States behind their parents: slot b * beams + k of dst = slot b * beams + parents[b][k] of src, for each of n_parts pieces of state.  A piece
+ * is `outer` x `segs` runs of seg_bytes bytes in every slot, run (i, j) at slot * slot_stride + i * outer_stride + j * seg_stride
+ * (bytes).  dst == src with equal strides: in place (only what changes its slot is read and written); else the two share no memory.  A parent
+ * outside [0, beams): the slot itself.  1 <= beams <= MD_MAX_BEAMS. */
+typedef struct {
+  const void* src;
+  void* dst;
+  int64_t src_slot_stride, dst_slot_stride, src_outer_stride, dst_outer_stride, src_seg_stride, dst_seg_stride, seg_bytes;
+  int32_t outer, segs;
+} md_state_part;
+md_status md_state_reorder(const md_state_part* parts, int32_t n_parts, const int32_t* parents, int32_t batch, int32_t beams, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

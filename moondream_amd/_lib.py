@@ -18,12 +18,12 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libmoondream_hip.so")
 SOURCES = ["gemm_bf16.hip", "gemm_w4.hip", "gemm_mid.hip", "gemm_fp8w.hip", "gemm_f8.hip", "quant_f8.hip", "attention_f8kv.hip", "decode_b1.hip", "attention.hip",
            "elementwise.hip", "image_crops.hip", "sampling_region.hip", "api.hip", "abi.hip", "lm_ops.hip", "gemm_step.hip", "gemm_f32.hip", "attention_talk.hip", "retention.hip",
-           "attention_latent.hip", "state_space.hip", "experts.hip", "gemm_experts.hip", "streams.hip", "lm_api.hip"]
+           "attention_latent.hip", "state_space.hip", "experts.hip", "gemm_experts.hip", "streams.hip", "lm_api.hip", "block_cache.hip", "attention_blocks.hip", "beams.hip"]
 # the part of the library that the layered language models use: a checkout that serves only such a model compiles no more
 LM_LIB_PATH = os.path.join(HERE, "libmoondream_lm.so")
 LM_SOURCES = ["gemm_bf16.hip", "gemm_w4.hip", "gemm_mid.hip", "elementwise.hip", "sampling_region.hip", "abi.hip", "lm_ops.hip", "gemm_step.hip", "gemm_f32.hip", "attention_talk.hip",
               "retention.hip", "attention_latent.hip", "state_space.hip", "experts.hip", "gemm_experts.hip", "streams.hip", "lm_api.hip"]
-HEADERS = ["md_common.hpp", "gemm_internal.hpp", "stage_common.hpp", "lm_internal.hpp", "step_weights.hpp"]
+HEADERS = ["md_common.hpp", "gemm_internal.hpp", "stage_common.hpp", "lm_internal.hpp", "step_weights.hpp", "block_cache.hpp"]
 
 MD_OK = 0
 ABI_VERSION = 5  # include/moondream_hip.h MD_ABI_VERSION
@@ -197,6 +197,44 @@ class MdLmBatch(C.Structure):
                 ("ctx_rows", c_int32), ("seq_ctx0", c_void_p)]
 
 
+MD_KV8_BLOCK, MD_KV8_MIN_EXP, MD_KV8_MAX_EXP = 32, -40, 40
+MD_MAX_BEAMS = 16
+
+
+class MdKv8Cache(C.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_exp", c_void_p), ("v_exp", c_void_p), ("slot_stride", c_int64), ("exp_stride", c_int64),
+                ("slots", c_int32), ("ctx", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32)]
+
+
+class MdKv8AttnArgs(C.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("q_bs", c_int64), ("q_ts", c_int64), ("q_hs", c_int64), ("o", c_void_p), ("o_bs", c_int64), ("o_ts", c_int64),
+        ("o_hs", c_int64), ("batch", c_int32), ("n_heads", c_int32), ("q_len", c_int32), ("slot", c_void_p), ("q_pos0", c_void_p),
+        ("q_rows", c_void_p), ("kv_len", c_void_p), ("max_len", c_int32), ("prefix_len", c_int32), ("scale", c_float), ("decay", c_float),
+        ("weights", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class MdKv8EvictArgs(C.Structure):
+    _fields_ = [("weights", c_void_p), ("weights_out", c_void_p), ("slot", c_void_p), ("kv_len", c_void_p), ("len_out", c_void_p),
+                ("kept", c_void_p), ("batch", c_int32), ("keep", c_int32), ("first", c_int32), ("recent", c_int32)]
+
+
+class MdBeamArgs(C.Structure):
+    _fields_ = [
+        ("logits", c_void_p), ("ld", c_int64), ("dtype", c_int32), ("batch", c_int32), ("beams", c_int32), ("vocab", c_int32),
+        ("suppress_id", c_int32), ("end_id", c_int32), ("scores", c_void_p), ("ended", c_void_p), ("rank_weight", c_void_p),
+        ("tokens", c_void_p), ("parents", c_void_p), ("scores_out", c_void_p), ("ended_out", c_void_p), ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+    ]
+
+
+class MdStatePart(C.Structure):
+    _fields_ = [("src", c_void_p), ("dst", c_void_p), ("src_slot_stride", c_int64), ("dst_slot_stride", c_int64), ("src_outer_stride", c_int64),
+                ("dst_outer_stride", c_int64), ("src_seg_stride", c_int64), ("dst_seg_stride", c_int64), ("seg_bytes", c_int64),
+                ("outer", c_int32), ("segs", c_int32)]
+
+
 # name -> (restype, argtypes): every symbol include/moondream_hip.h declares
 P = C.POINTER
 SIGNATURES = {
@@ -279,6 +317,15 @@ SIGNATURES = {
     "md_argmax_f32": (C.c_int, [c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
     "md_gemm_f32": (C.c_int, [c_void_p, c_int64, P(MdLinear), c_void_p, c_int64, c_int32, c_void_p]),
     "md_lm_set_kernels": (None, [c_int32]),
+    "md_kv8_append": (C.c_int, [P(MdKv8Cache), c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                c_void_p, c_int32, c_int32, c_void_p]),
+    "md_kv8_read": (C.c_int, [P(MdKv8Cache), c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
+    "md_kv8_attention_workspace_bytes": (c_size_t, [P(MdKv8Cache), P(MdKv8AttnArgs)]),
+    "md_kv8_attention": (C.c_int, [P(MdKv8Cache), P(MdKv8AttnArgs), c_void_p]),
+    "md_kv8_evict": (C.c_int, [P(MdKv8Cache), P(MdKv8Cache), P(MdKv8EvictArgs), c_void_p]),
+    "md_beam_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32]),
+    "md_beam_select": (C.c_int, [P(MdBeamArgs), c_void_p]),
+    "md_state_reorder": (C.c_int, [P(MdStatePart), c_int32, c_void_p, c_int32, c_int32, c_void_p]),
     "md_decode_workspace_bytes": (c_size_t, [P(MdTextModel), c_int32]),
     "md_decode_step": (C.c_int, [P(MdTextModel), c_void_p, c_void_p, c_void_p, c_int32, P(MdKvCache), c_int32,
                                  c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),

@@ -1,0 +1,120 @@
+"""Beam search on the device: the choice among all beams' continuations, and the beams' states moved behind their parents.
+
+    choice = select_beams(logits, scores, ended=ended, end_id=eos)     # [batch * beams, vocab] -> tokens, parents, scores, ended
+    reorder_states([k_slab, v_slab], choice.parents, slot_dim=1)       # the caches of all layers, in place
+
+A search starts with all scores but the first of every input -inf: the first step then takes the best tokens of one beam.  Both run on the
+current stream of their tensors' device, allocate through torch only, never synchronise and can be captured into a graph.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional, Sequence
+
+import torch
+
+from . import _lib
+from .block_cache import _need, _on, _stream
+
+MAX_BEAMS = _lib.MD_MAX_BEAMS
+_DTYPES = {torch.bfloat16: _lib.MD_DTYPE_BF16, torch.float32: _lib.MD_DTYPE_F32}
+
+
+class BeamChoice(NamedTuple):
+    tokens: torch.Tensor   # int32 [batch, beams]
+    parents: torch.Tensor  # int32 [batch, beams]: the beam, of the same input, that the token goes on from
+    scores: torch.Tensor   # fp32 [batch, beams], falling (by rank)
+    ended: torch.Tensor    # int32 [batch, beams]
+
+
+def _gpu(t: torch.Tensor, what: str) -> torch.device:
+    if t.device.type != "cuda":
+        raise _lib.MoondreamHipError(f"{what} needs a GPU device; there is no CPU path")
+    return t.device
+
+
+def select_beams(logits: torch.Tensor, scores: torch.Tensor, ended: Optional[torch.Tensor] = None, end_id: int = -1, suppress_id: int = -1,
+                 rank_weight: Optional[torch.Tensor] = None) -> BeamChoice:
+    """The ``beams`` best continuations of every input's beams.  ``logits`` [batch * beams, vocab] (bf16 or fp32, rows may lie apart), ``scores`` fp32
+    [batch, beams]: a beam's sum of log probabilities so far, -inf for one that does not exist.  ``ended`` (int32 [batch, beams]): beams that have ended
+    stay in the running with their score, as one continuation ``end_id``.  ``rank_weight`` (fp32 [batch, beams], > 0) multiplies the totals of a beam's
+    continuations for the choice alone (a length penalty: 1 / length ** alpha).  Ties: the lower beam, the larger logit, the lower token.
+    Where fewer than ``beams`` continuations are left: token ``end_id``, score -inf, ended, its own parent."""
+    if scores.dim() != 2 or logits.dim() != 2 or logits.shape[0] != scores.shape[0] * scores.shape[1] or logits.dtype not in _DTYPES or logits.shape[1] == 0:
+        raise ValueError(f"logits {tuple(logits.shape)} {logits.dtype} for scores {tuple(scores.shape)}: wanted [batch * beams, vocab] bfloat16 or float32")
+    batch, beams = scores.shape
+    vocab = logits.shape[1]
+    if not 2 <= beams <= MAX_BEAMS or batch == 0:
+        raise ValueError(f"{batch} inputs of {beams} beams: wanted 2 to {MAX_BEAMS} beams")
+    if end_id >= vocab or (end_id < 0 and ended is not None):
+        raise ValueError(f"end_id {end_id} of {vocab} tokens" + (" with ended beams" if ended is not None else ""))
+    if logits.stride(1) != 1 or logits.stride(0) < vocab:
+        raise ValueError(f"logits of strides {logits.stride()}: rows have to be contiguous and apart")
+    dev, shape = _gpu(logits, "select_beams"), (batch, beams)
+    addresses = [None if t is None else _need(t, name, dtype, dev, shape)
+                 for t, name, dtype in ((scores, "scores", torch.float32), (ended, "ended", torch.int32), (rank_weight, "rank_weight", torch.float32))]
+    ints = torch.empty(3, batch, beams, dtype=torch.int32, device=dev)
+    new = torch.empty(shape, dtype=torch.float32, device=dev)
+    tokens, parents, stop = ints.unbind(0)
+    lib = _lib.load()
+    with _on(dev):
+        need = lib.md_beam_workspace_bytes(batch, beams, vocab)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        a = _lib.MdBeamArgs(logits.data_ptr(), logits.stride(0), _DTYPES[logits.dtype], batch, beams, vocab, suppress_id, max(end_id, -1), *addresses,
+                            tokens.data_ptr(), parents.data_ptr(), new.data_ptr(), stop.data_ptr(), ws.data_ptr(), need)
+        _lib.check(lib.md_beam_select(C.byref(a), _stream(dev)), "md_beam_select")
+    return BeamChoice(tokens, parents, new, stop)
+
+
+def _runs(t: torch.Tensor, slot_dim: int, name: str):
+    """(slot stride, outer count and stride, run count and stride, run length), in bytes, of a tensor's slots."""
+    size = t.element_size()
+    dims = [(n, s * size) for d, (n, s) in enumerate(zip(t.shape, t.stride())) if d != slot_dim and n > 1]
+    length = size
+    while dims and dims[-1][1] == length:
+        length *= dims.pop()[0]
+    joined = []
+    for n, s in dims:  # neighbours that are one dimension in memory
+        if joined and joined[-1][1] == n * s:
+            joined[-1] = (joined[-1][0] * n, s)
+        else:
+            joined.append((n, s))
+    if len(joined) > 2:
+        raise ValueError(f"{name}: strides {t.stride()} leave more than two dimensions that lie apart")
+    outer, segs = ([(1, 0)] * 2 + joined)[-2:]
+    return t.stride(slot_dim) * size, outer, segs, length
+
+
+def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, into: Optional[Sequence[torch.Tensor]] = None, slot_dim: int = 0) -> None:
+    """Slot b * beams + k of every state <- its slot b * beams + parents[b, k] (``parents``: int32 [batch, beams]), in place, or from ``states`` to ``into``
+    (tensors of the same shapes and types that share no memory with them).  ``slot_dim``: the states' dimension of slots; the first batch * beams
+    slots take part.  States may be views -- the rows of an answer in all layers' slabs, ``slab[:, :, :, first:last]`` -- whose dimensions
+    besides the slots' make at most two strides apart.  What lies in front of the answers is the same for all beams of an input and need not be moved."""
+    if parents.dim() != 2 or not 1 <= parents.shape[1] <= MAX_BEAMS or parents.shape[0] == 0:
+        raise ValueError(f"parents {tuple(parents.shape)}: wanted [batch, 1 to {MAX_BEAMS} beams]")
+    batch, beams = parents.shape
+    into = states if into is None else into
+    if len(into) != len(states):
+        raise ValueError(f"{len(states)} states into {len(into)}")
+    parts = []
+    for i, (src, dst) in enumerate(zip(states, into)):
+        name = f"state {i}"
+        if src.shape != dst.shape or src.dtype != dst.dtype or src.device != parents.device or dst.device != parents.device:
+            raise ValueError(f"{name}: {tuple(src.shape)} {src.dtype} on {src.device} into {tuple(dst.shape)} {dst.dtype} on {dst.device}")
+        if not -src.dim() <= slot_dim < src.dim() or src.shape[slot_dim] < batch * beams:
+            raise ValueError(f"{name}: {tuple(src.shape)} has fewer than {batch * beams} slots in dimension {slot_dim}")
+        if src.numel() == 0:
+            continue
+        at = slot_dim % src.dim()
+        a = _runs(src, at, name)
+        b = a if src is dst else _runs(dst, at, name)
+        if (a[1][0], a[2][0], a[3]) != (b[1][0], b[2][0], b[3]):
+            raise ValueError(f"{name}: strides {src.stride()} into {dst.stride()}")
+        parts.append((src.data_ptr(), dst.data_ptr(), a[0], b[0], a[1][1], b[1][1], a[2][1], b[2][1], a[3], a[1][0], a[2][0]))
+    if not parts:
+        return
+    dev = _gpu(parents, "reorder_states")
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check(lib.md_state_reorder((_lib.MdStatePart * len(parts))(*parts), len(parts), _need(parents, "parents", torch.int32, dev), batch, beams,
+                                        _stream(dev)), "md_state_reorder")

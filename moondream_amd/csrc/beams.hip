@@ -1,0 +1,346 @@
+// Beam search: the best continuations over beams and vocabulary, and states moved behind their parents.
+//
+//   total(k, t) = score_k + logit_t - log sum_v exp(logit_v)
+// Within a beam totals follow the logits, so a beam's candidates are its `beams` largest logits (ties: the lower token): one pass over the
+// logits gives them and the sum, and only beams x beams totals are ever compared.
+//   part_kernel    one workgroup per (beam, piece of the vocabulary): the piece in registers; each wave's largest logits one after another
+//                  (only the lane that gave one looks for its next), its maximum and its sum of exponentials
+//   choose_kernel  one workgroup per input: sums joined in 64 bits, every beam's candidates, totals, their order by counting who is ahead
+// Bound by the logits' bytes; with few rows by the two launches.
+#include "md_common.hpp"
+
+#include <algorithm>
+
+namespace {
+
+constexpr int PIECE = 8192;  // logits of a workgroup: 32 per thread
+constexpr int PER = PIECE / 256;
+constexpr int MAXB = MD_MAX_BEAMS;
+constexpr float F32_MOST = 3.4028234663852886e38f;
+
+// (value, index) as one number: the larger value first, of equal ones the lower index.  0 stands for nothing.
+__device__ __forceinline__ uint64_t candidate(float v, uint32_t index) {
+  v = v == 0.f ? 0.f : v;  // -0 and 0 are equal
+  const uint32_t u = __float_as_uint(v), o = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return ((uint64_t)o << 32) | (uint32_t)~index;
+}
+__device__ __forceinline__ float value_of(uint64_t c) {
+  const uint32_t o = (uint32_t)(c >> 32);
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+__device__ __forceinline__ uint32_t index_of(uint64_t c) { return ~(uint32_t)c; }
+
+__device__ __forceinline__ uint64_t wave_most(uint64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint64_t w = __shfl_xor((unsigned long long)v, o, 64);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+
+// a beam that has continuations of its own
+__device__ __forceinline__ bool goes_on(const float* scores, const int32_t* ended, int row) {
+  return scores[row] > -INFINITY && (!ended || ended[row] == 0);
+}
+
+template <typename T>
+__device__ __forceinline__ float logit(T x);
+template <>
+__device__ __forceinline__ float logit<bf16_t>(bf16_t x) { return bf2f(x); }
+template <>
+__device__ __forceinline__ float logit<float>(float x) { return x; }
+
+template <typename T>
+__global__ __launch_bounds__(256) void part_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int beams, int suppress_id,
+                                                   const float* __restrict__ scores, const int32_t* __restrict__ ended, int pieces,
+                                                   uint64_t* __restrict__ best, double* __restrict__ sums) {
+  constexpr int E = 16 / sizeof(T), N = PER / E;  // elements of a load, loads of a thread
+  __shared__ uint64_t lists[4 * MAXB];
+  __shared__ float wmax[4];
+  __shared__ double wsum[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, piece = blockIdx.x, row = blockIdx.y;
+  if (!goes_on(scores, ended, row)) return;
+  const T* x = logits + (int64_t)row * ld;
+  const int base = piece * PIECE;
+  const bool aligned = ((uintptr_t)x & 15) == 0;
+  float v[PER];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int at = base + (i * 256 + (int)threadIdx.x) * E;
+    if (aligned && at + E <= vocab) {
+      const u32x4 w = *(const u32x4*)(x + at);
+      const T* e = (const T*)&w;
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[i * E + j] = logit<T>(e[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[i * E + j] = at + j < vocab ? logit<T>(x[at + j]) : -INFINITY;
+    }
+  }
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int id = base + ((i / E) * 256 + (int)threadIdx.x) * E + i % E;
+    v[i] = v[i] == v[i] && id != suppress_id ? fminf(v[i], F32_MOST) : -INFINITY;
+    top = fmaxf(top, v[i]);
+  }
+  const float m = wave_max(top);
+  double sum = 0.;
+  if (m > -INFINITY) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += (double)expf(v[i] - m);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+
+  uint64_t taken = ~0ull, mine = 0;
+  const auto next = [&]() {  // this thread's largest below what it gave last
+    mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const uint64_t c = candidate(v[i], base + ((i / E) * 256 + (int)threadIdx.x) * E + i % E);
+      if (v[i] > -INFINITY && c < taken && c > mine) mine = c;
+    }
+  };
+  next();
+  for (int k = 0; k < beams; ++k) {
+    const uint64_t c = wave_most(mine);
+    if (lane == 0) lists[wave * beams + k] = c;
+    if (c != 0 && c == mine) {
+      taken = c;
+      next();
+    }
+  }
+  if (lane == 0) {
+    wmax[wave] = m;
+    wsum[wave] = sum;
+  }
+  __syncthreads();
+  if (wave == 0) {  // of at most 64 the largest, one per lane, each at the place that counting gives it
+    const int n = 4 * beams;
+    const uint64_t c = lane < n ? lists[lane] : 0;
+    int ahead = 0;
+    for (int j = 0; j < n; ++j) ahead += lists[j] > c || (lists[j] == c && j < lane);
+    if (lane < n && ahead < beams) best[((int64_t)row * pieces + piece) * beams + ahead] = c;
+    if (lane == 0) {
+      const float mm = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+      double s = 0.;
+      for (int w = 0; w < 4; ++w)
+        if (wmax[w] > -INFINITY) s += wsum[w] * exp((double)wmax[w] - (double)mm);
+      sums[((int64_t)row * pieces + piece) * 2] = (double)mm;
+      sums[((int64_t)row * pieces + piece) * 2 + 1] = s;
+    }
+  }
+}
+
+struct Ranked {
+  double rank;
+  uint64_t logit;  // candidate(): the logit and its token
+};
+
+__global__ __launch_bounds__(256) void choose_kernel(int beams, int pieces, int end_id, const float* scores, const int32_t* ended,
+                                                     const float* __restrict__ rank_weight, const uint64_t* __restrict__ best,
+                                                     const double* __restrict__ sums, int32_t* __restrict__ tokens, int32_t* __restrict__ parents,
+                                                     float* scores_out, int32_t* ended_out) {
+  __shared__ Ranked cand[MAXB * MAXB];
+  __shared__ double totals[MAXB * MAXB];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.x, row0 = b * beams, n = beams * beams;
+  for (int k = wave; k < beams; k += 4) {
+    const int row = row0 + k;
+    const float score = scores[row], weight = rank_weight ? rank_weight[row] : 1.f;
+    if (!goes_on(scores, ended, row)) {  // (an ended beam of a score: itself, and nothing else)
+      if (lane < beams) {
+        const bool itself = lane == 0 && score > -INFINITY;
+        cand[k * beams + lane] = {itself ? (double)score * (double)weight : -INFINITY, itself ? candidate(0.f, end_id) : 0};
+        totals[k * beams + lane] = itself ? (double)score : -INFINITY;
+      }
+      continue;
+    }
+    double m = -INFINITY, s = 0.;
+    for (int i = 0; i < pieces; ++i) m = fmax(m, sums[((int64_t)row * pieces + i) * 2]);
+    for (int i = lane; i < pieces; i += 64) {
+      const double pm = sums[((int64_t)row * pieces + i) * 2];
+      if (pm > -INFINITY) s += sums[((int64_t)row * pieces + i) * 2 + 1] * exp(pm - m);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    const double norm = m + log(s);
+    const uint64_t* list = best + (int64_t)row * pieces * beams;
+    uint64_t taken = ~0ull;
+    for (int j = 0; j < beams; ++j) {
+      uint64_t c = 0;
+      for (int i = lane; i < pieces * beams; i += 64) {
+        const uint64_t e = list[i];
+        if (e < taken && e > c) c = e;
+      }
+      c = wave_most(c);
+      taken = c;
+      if (lane == 0) {
+        const double total = c ? (double)score + ((double)value_of(c) - norm) : -INFINITY;
+        const bool real = total > -INFINITY;
+        cand[k * beams + j] = {real ? total * (double)weight : -INFINITY, real ? c : 0};
+        totals[k * beams + j] = real ? total : -INFINITY;
+      }
+    }
+  }
+  __syncthreads();
+  // (every input of this input's beams has been read: what follows may overwrite scores and ended)
+  const int i = threadIdx.x;
+  const Ranked me = i < n ? cand[i] : Ranked{-INFINITY, 0};
+  const int parent = i / beams;
+  int was_ended = 0;
+  if (i < n) was_ended = ended && ended[row0 + parent] != 0;
+  int live = 0, ahead = 0;
+  for (int j = 0; j < n; ++j) {
+    const Ranked o = cand[j];
+    live += o.logit != 0;
+    ahead += o.logit != 0 && (o.rank > me.rank || (o.rank == me.rank && (j / beams < parent || (j / beams == parent && o.logit > me.logit))));
+  }
+  __syncthreads();
+  if (i < n && me.logit != 0 && ahead < beams) {
+    const int token = (int)index_of(me.logit), at = row0 + ahead;
+    tokens[at] = token;
+    parents[at] = parent;
+    scores_out[at] = (float)totals[i];
+    if (ended_out) ended_out[at] = was_ended || token == end_id;
+  }
+  if (i < beams && i >= live) {
+    tokens[row0 + i] = end_id;
+    parents[row0 + i] = i;
+    scores_out[row0 + i] = -INFINITY;
+    if (ended_out) ended_out[row0 + i] = 1;
+  }
+}
+
+size_t pieces_of(int vocab) { return ((size_t)vocab + PIECE - 1) / PIECE; }
+
+// ------------------------------------------------------------------------------------------------------------- states
+constexpr int MAX_PARTS = 32;  // of a launch (80 bytes each in its arguments)
+
+struct Part {
+  const char* src;
+  char* dst;
+  int64_t src_slot, dst_slot, src_outer, dst_outer, src_seg, dst_seg;
+  int32_t per_seg, segs;   // words of a run, runs of an outer index
+  int32_t first, width;    // the part's first workgroup; bytes of a word
+  int64_t words;
+};
+struct Parts {
+  Part p[MAX_PARTS];
+  int n;
+};
+
+template <typename W, int B>
+__device__ __forceinline__ void move_words(const Part& p, int64_t first, const int32_t* par, int beams, int64_t slot0) {
+  const int64_t w = first + threadIdx.x;
+  if (w >= p.words) return;
+  const int64_t run = w / p.per_seg;
+  const int in = (int)(w - run * p.per_seg), seg = (int)(run % p.segs);
+  const int64_t outer = run / p.segs;
+  const char* src = p.src + slot0 * p.src_slot + outer * p.src_outer + seg * p.src_seg + (int64_t)in * sizeof(W);
+  char* dst = p.dst + slot0 * p.dst_slot + outer * p.dst_outer + seg * p.dst_seg + (int64_t)in * sizeof(W);
+  const bool in_place = p.src == p.dst;
+  W v[B];
+#pragma unroll
+  for (int i = 0; i < B; ++i)
+    if (i < beams && !(in_place && par[i] == i)) v[i] = *(const W*)(src + par[i] * p.src_slot);
+#pragma unroll
+  for (int i = 0; i < B; ++i)
+    if (i < beams && !(in_place && par[i] == i)) *(W*)(dst + i * p.dst_slot) = v[i];
+}
+
+// One thread per word of a slot, for all beams of an input: every word is read from all parents before it is written to any child, so in place
+// needs no second copy and no order among workgroups.
+template <int B>
+__global__ __launch_bounds__(256) void reorder_kernel(Parts parts, const int32_t* __restrict__ parents, int beams) {
+  __shared__ int32_t par[B];
+  int i = 0;
+  while (i + 1 < parts.n && (int)blockIdx.x >= parts.p[i + 1].first) ++i;
+  const Part& p = parts.p[i];
+  const int b = blockIdx.y;
+  if ((int)threadIdx.x < beams) {
+    const int q = parents[(int64_t)b * beams + threadIdx.x];
+    par[threadIdx.x] = q >= 0 && q < beams ? q : threadIdx.x;
+  }
+  __syncthreads();
+  const int64_t first = (int64_t)((int)blockIdx.x - p.first) * 256;
+  if (p.width == 16) move_words<u32x4, B>(p, first, par, beams, (int64_t)b * beams);
+  else if (p.width == 4) move_words<uint32_t, B>(p, first, par, beams, (int64_t)b * beams);
+  else move_words<uint8_t, B>(p, first, par, beams, (int64_t)b * beams);
+}
+
+int64_t extent(const md_state_part& s, bool src, int64_t slots) {
+  const int64_t a = src ? s.src_slot_stride : s.dst_slot_stride, b = src ? s.src_outer_stride : s.dst_outer_stride, c = src ? s.src_seg_stride : s.dst_seg_stride;
+  return (slots - 1) * a + (s.outer - 1) * b + (s.segs - 1) * c + s.seg_bytes;
+}
+
+bool part_ok(const md_state_part& s, int64_t slots) {
+  if (!s.src || !s.dst || s.seg_bytes <= 0 || s.outer <= 0 || s.segs <= 0) return false;
+  const int64_t strides[6] = {s.src_slot_stride, s.dst_slot_stride, s.src_outer_stride, s.dst_outer_stride, s.src_seg_stride, s.dst_seg_stride};
+  for (int64_t x : strides)
+    if (x < 0) return false;
+  if ((s.dst_slot_stride < s.seg_bytes && slots > 1) || (s.dst_outer_stride < s.seg_bytes && s.outer > 1) || (s.dst_seg_stride < s.seg_bytes && s.segs > 1))
+    return false;  // (two runs would be written to one place)
+  if (s.src == s.dst) return s.src_slot_stride == s.dst_slot_stride && s.src_outer_stride == s.dst_outer_stride && s.src_seg_stride == s.dst_seg_stride;
+  const uintptr_t a = (uintptr_t)s.src, b = (uintptr_t)s.dst;
+  return a + (uintptr_t)extent(s, true, slots) <= b || b + (uintptr_t)extent(s, false, slots) <= a;
+}
+
+}  // namespace
+
+extern "C" size_t md_beam_workspace_bytes(int32_t batch, int32_t beams, int32_t vocab) {
+  if (batch <= 0 || beams < 2 || beams > MAXB || vocab <= 0) return 0;
+  return (size_t)batch * beams * pieces_of(vocab) * (beams * sizeof(uint64_t) + 2 * sizeof(double));
+}
+
+extern "C" md_status md_beam_select(const md_beam_args* a, void* stream) {
+  MD_CHECK_ARG(a && a->logits && a->scores && a->tokens && a->parents && a->scores_out && a->batch > 0 && a->vocab > 0 && a->ld >= a->vocab);
+  MD_CHECK_ARG(a->beams >= 2 && a->beams <= MAXB && (a->dtype == MD_DTYPE_BF16 || a->dtype == MD_DTYPE_F32) && (int64_t)a->batch * a->beams <= 65535);
+  MD_CHECK_ARG(a->end_id < a->vocab && (a->end_id >= 0 || !a->ended) && ((uintptr_t)a->logits & (a->dtype == MD_DTYPE_F32 ? 3 : 1)) == 0);
+  const int pieces = (int)pieces_of(a->vocab), rows = a->batch * a->beams;
+  if (!a->workspace || a->workspace_bytes < md_beam_workspace_bytes(a->batch, a->beams, a->vocab)) return MD_ERR_WORKSPACE;
+  MD_CHECK_ARG(((uintptr_t)a->workspace & 15) == 0);
+  uint64_t* best = (uint64_t*)a->workspace;
+  double* sums = (double*)(best + (size_t)rows * pieces * a->beams);
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 grid(pieces, rows);
+  if (a->dtype == MD_DTYPE_BF16)
+    hipLaunchKernelGGL(part_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t*)a->logits, a->ld, a->vocab, a->beams, a->suppress_id, a->scores, a->ended,
+                       pieces, best, sums);
+  else
+    hipLaunchKernelGGL(part_kernel<float>, grid, dim3(256), 0, s, (const float*)a->logits, a->ld, a->vocab, a->beams, a->suppress_id, a->scores, a->ended,
+                       pieces, best, sums);
+  hipLaunchKernelGGL(choose_kernel, dim3(a->batch), dim3(256), 0, s, a->beams, pieces, a->end_id, a->scores, a->ended, a->rank_weight, best, sums,
+                     a->tokens, a->parents, a->scores_out, a->ended_out);
+  return md_launch_status();
+}
+
+extern "C" md_status md_state_reorder(const md_state_part* parts, int32_t n_parts, const int32_t* parents, int32_t batch, int32_t beams, void* stream) {
+  MD_CHECK_ARG(parts && n_parts > 0 && parents && batch > 0 && batch <= 65535 && beams > 0 && beams <= MAXB);
+  for (int i = 0; i < n_parts; ++i) MD_CHECK_ARG(part_ok(parts[i], (int64_t)batch * beams));
+  for (int done = 0; done < n_parts;) {
+    Parts ps;
+    ps.n = 0;
+    int64_t groups = 0;
+    for (; done < n_parts && ps.n < MAX_PARTS; ++done) {
+      const md_state_part& s = parts[done];
+      const uint64_t all = (uint64_t)s.src | (uint64_t)s.dst | (uint64_t)s.src_slot_stride | (uint64_t)s.dst_slot_stride | (uint64_t)s.src_outer_stride |
+                           (uint64_t)s.dst_outer_stride | (uint64_t)s.src_seg_stride | (uint64_t)s.dst_seg_stride | (uint64_t)s.seg_bytes;
+      const int width = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+      const int64_t per = s.seg_bytes / width, words = per * s.segs * s.outer, mine = (words + 255) / 256;
+      MD_CHECK_ARG(per <= 0x7fffffff && mine <= 0x7fffffff);
+      if (groups + mine > 0x7fffffff) break;
+      ps.p[ps.n++] = {(const char*)s.src, (char*)s.dst, s.src_slot_stride, s.dst_slot_stride, s.src_outer_stride, s.dst_outer_stride, s.src_seg_stride,
+                      s.dst_seg_stride, (int32_t)per, s.segs, (int32_t)groups, width, words};
+      groups += mine;
+    }
+    const dim3 grid((unsigned)groups, batch);
+    hipStream_t st = (hipStream_t)stream;
+    if (beams <= 4) hipLaunchKernelGGL(reorder_kernel<4>, grid, dim3(256), 0, st, ps, parents, beams);
+    else if (beams <= 8) hipLaunchKernelGGL(reorder_kernel<8>, grid, dim3(256), 0, st, ps, parents, beams);
+    else hipLaunchKernelGGL(reorder_kernel<16>, grid, dim3(256), 0, st, ps, parents, beams);
+    MD_TRY(md_launch_status());
+  }
+  return MD_OK;
+}

@@ -15,7 +15,7 @@
 // m moves only when a column's exponent exceeds it by more than 8 (P <= 2^8): mostly one comparison instead of a reduction and a rescaling.
 //
 // Few columns (decode): the four waves of a workgroup share a column tile and take every fourth block, several workgroups share the keys, and
-// a second kernel joins their (O, m, l).  Many columns (prompts): every wave has its own columns.
+// a second kernel joins their (O, m, l).  Many columns (prompts): every wave has its own columns, the converted operands come through LDS.
 #include "block_cache.hpp"
 
 #include <algorithm>
@@ -42,6 +42,8 @@ struct Params {
   int64_t o_bs, o_ts, o_hs;
   const int32_t *slot, *q_pos0, *q_rows, *kv_len;
   int group, q_len, max_len, prefix, splits, col_groups, cols;
+  uint32_t per_group, all;  // 2^32 / group rounded up and 0; 0 and ~0 for a group of 1
+  uint32_t q_sign;          // xor of two bf16 queries: a negative scale is taken as its magnitude and the queries negated, so that scores rise with products
   float scale_log2, decay;
   float *part, *part_ml, *lse, *weights;  // part: [batch][kv_heads][cols][splits][head_dim], part_ml: ... [splits][2], lse: [batch][kv_heads][cols]
 };
@@ -59,6 +61,9 @@ __device__ __forceinline__ Seq sequence(const Params& p, int b) {
   s.pos0 = p.q_pos0 ? min(max(p.q_pos0[b], -p.q_len), p.max_len) : s.len - s.rows;
   return s;
 }
+// column -> query (exact: columns * group < 2^32)
+__device__ __forceinline__ int query_of(const Params& p, int col) { return (int)(__umulhi((uint32_t)col, p.per_group) + ((uint32_t)col & p.all)); }
+
 // how many keys the query in row `pos` sees
 __device__ __forceinline__ int limit_of(const Params& p, const Seq& s, int pos) {
   const int n = pos < 0 ? 0 : (pos < p.prefix ? max(pos + 1, p.prefix) : pos + 1);
@@ -130,25 +135,34 @@ __device__ __forceinline__ void transpose4(const uint32_t (&w)[4], uint32_t (&ou
   out[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
 
-// the scores' product: 32 keys x 16 columns
-template <int HD>
-__device__ __forceinline__ void scores(const bf16x8 (&a)[2][HD / 32], const bf16x8 (&qf)[HD / 32], f32x4 (&s)[2]) {
+// the scores' product: KT tiles of 16 keys x NT of 16 columns, the independent accumulators in turn
+template <int HD, int KT, int NT>
+__device__ __forceinline__ void scores(const bf16x8 (&a)[KT][HD / 32], const bf16x8 (&qf)[NT][HD / 32], f32x4 (&s)[NT][KT]) {
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
-    for (int c = 0; c < HD / 32; ++c) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a[t][c]), __builtin_bit_cast(b16x8, qf[c]), s[t], 0, 0, 0);
-  }
+    for (int t = 0; t < KT; ++t) s[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < HD / 32; ++c)
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct)
+        s[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a[t][c]), __builtin_bit_cast(b16x8, qf[ct][c]), s[ct][t], 0, 0, 0);
+}
+
+__device__ __forceinline__ bf16x8 query_at(const Params& p, const bf16_t* at) {
+  return __builtin_bit_cast(bf16x8, *(const u32x4*)at ^ u32x4{p.q_sign, p.q_sign, p.q_sign, p.q_sign});
 }
 
 // a column's query as the scores' second operand: coordinates in the order in which a lane's bytes of a key hold them
 template <int HD>
 __device__ __forceinline__ void load_query(const Params& p, int b, int kvh, int col, int rows, int q, bf16x8 (&qf)[HD / 32]) {
-  const int t = col / p.group, g = col - t * p.group;
+  const int t = query_of(p, col), g = col - t * p.group;
 #pragma unroll
   for (int c = 0; c < HD / 32; ++c) {
     qf[c] = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
-    if (t < rows) qf[c] = *(const bf16x8*)(p.q + (int64_t)b * p.q_bs + (int64_t)t * p.q_ts + (int64_t)(kvh * p.group + g) * p.q_hs + (c >> 1) * 64 + q * 16 + (c & 1) * 8);
+    if (t < rows) qf[c] = query_at(p, p.q + (int64_t)b * p.q_bs + (int64_t)t * p.q_ts + (int64_t)(kvh * p.group + g) * p.q_hs + (c >> 1) * 64 + q * 16 + (c & 1) * 8);
   }
 }
 
@@ -161,28 +175,93 @@ __device__ __forceinline__ float over_q_max(float v) {
   return fmaxf(v, __shfl_xor(v, 32, 64));
 }
 
-// WK: waves of a workgroup that share columns and take the key blocks in turn; the other 4 / WK have columns of their own.
-template <int HD, int NT, int WK>
-__global__ __launch_bounds__(256) void attention_kernel(Params p) {
-  constexpr int VT = HD / 16;  // tiles of 16 coordinates of the output
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-  const int split = blockIdx.x % p.splits, cg = blockIdx.x / p.splits, kvh = blockIdx.y, b = blockIdx.z;
-  const Seq sq = sequence(p, b);
-  const int n_cols = sq.rows * p.group;
-  const int col0 = (cg * (4 / WK) + wave / WK) * 16 * NT;
-  if constexpr (WK == 1) {
-    if (col0 >= n_cols) return;
-  } else {
-    if (cg * 16 * NT >= n_cols) return;  // (all four waves)
+// One block's softmax for NT tiles of columns: scores s -> pf, P as the second product's operand; m, l and acc move with it.  `edge`: some column does
+// not see all of the block.
+template <int NT, int VT>
+__device__ __forceinline__ void softmax_block(f32x4 (&s)[NT][2], f16x8 (&pf)[NT], f32x4 (&acc)[NT][VT], float (&m)[NT], float (&l)[NT], const int (&lim)[NT],
+                                              bool edge, int key0, int q, float ck, float ev, float back) {
+  if (edge) {
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (key0 + t * 16 + 4 * q + i >= lim[ct]) s[ct][t][i] = -INFINITY;
   }
-
-  bf16x8 qf[NT][HD / 32];
-  int lim[NT], most = 0, least = 0x7fffffff;
+  float top[NT];
+  bool over = false;
 #pragma unroll
   for (int ct = 0; ct < NT; ++ct) {
-    const int col = col0 + ct * 16 + r;
-    load_query<HD>(p, b, kvh, col, sq.rows, q, qf[ct]);
-    lim[ct] = col < n_cols ? limit_of(p, sq, sq.pos0 + col / p.group) : 0;
+    float a = s[ct][0][0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) a = fmaxf(a, s[ct][j >> 2][j & 3]);
+    top[ct] = __builtin_fmaf(a, ck, ev);
+    over |= top[ct] > m[ct] + SLACK;
+  }
+  if (__any(over)) {
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) {
+      const float now = fmaxf(m[ct], over_q_max(top[ct])), f0 = __builtin_amdgcn_exp2f(m[ct] - now);
+      m[ct] = now;
+      l[ct] *= f0;
+#pragma unroll
+      for (int t = 0; t < VT; ++t) acc[ct][t] *= f0;
+    }
+  }
+#pragma unroll
+  for (int ct = 0; ct < NT; ++ct) {
+    const float shift = ev - m[ct];
+    float sum = 0.f, e[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ct][j >> 2][j & 3], ck, shift));
+      sum += e[j];
+    }
+    l[ct] = __builtin_fmaf(sum, back, l[ct]);
+    union {
+      f16x2 h[4];
+      f16x8 v;
+    } u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u.h[j] = __builtin_convertvector((md_f32pair{e[2 * j], e[2 * j + 1]}), f16x2);
+    pf[ct] = u.v;
+  }
+}
+
+// Writes column `col`'s coordinates at0 .. of a split, or its output; o[n] unnormalised
+template <int HD, int N>
+__device__ __forceinline__ void store_column(const Params& p, int b, int kvh, int col, int split, int at0, const float (&o)[N], float m, float l, bool first) {
+  const int64_t c = ((int64_t)b * p.kv_heads + kvh) * p.cols + col;
+  if (p.splits > 1) {
+    float* out = p.part + (c * p.splits + split) * HD + at0;
+#pragma unroll
+    for (int i = 0; i < N; i += 4) *(f32x4*)(out + i) = f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
+    if (first) {
+      p.part_ml[(c * p.splits + split) * 2] = m;
+      p.part_ml[(c * p.splits + split) * 2 + 1] = l;
+    }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int t = query_of(p, col), g = col - t * p.group;
+  bf16_t* out = p.o + (int64_t)b * p.o_bs + (int64_t)t * p.o_ts + (int64_t)(kvh * p.group + g) * p.o_hs + at0;
+#pragma unroll
+  for (int i = 0; i < N; i += 4) *(u32x2*)(out + i) = u32x2{pack_bf16x2(o[i] * inv, o[i + 1] * inv), pack_bf16x2(o[i + 2] * inv, o[i + 3] * inv)};
+  if (p.lse && first) p.lse[c] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// The columns of a wave: queries, how many keys each sees, and the most and the least of them
+template <int HD, int NT>
+__device__ __forceinline__ void load_columns(const Params& p, const Seq& sq, int b, int kvh, int col0, int n_cols, int lane, bf16x8 (&qf)[NT][HD / 32], int (&lim)[NT],
+                                             int& most, int& least) {
+  most = 0;
+  least = 0x7fffffff;
+#pragma unroll
+  for (int ct = 0; ct < NT; ++ct) {
+    const int col = col0 + ct * 16 + (lane & 15);
+    load_query<HD>(p, b, kvh, col, sq.rows, lane >> 4, qf[ct]);
+    lim[ct] = col < n_cols ? limit_of(p, sq, sq.pos0 + query_of(p, col)) : 0;
     most = max(most, lim[ct]);
     if (col < n_cols) least = min(least, lim[ct]);
   }
@@ -193,7 +272,21 @@ __global__ __launch_bounds__(256) void attention_kernel(Params p) {
   }
   most = __builtin_amdgcn_readfirstlane(most);
   least = __builtin_amdgcn_readfirstlane(least);
+}
 
+// Few columns: the four waves share NT column tiles and take every fourth block, registers only.
+template <int HD, int NT>
+__global__ __launch_bounds__(256) void decode_kernel(Params p) {
+  constexpr int VT = HD / 16;  // tiles of 16 coordinates of the output
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int split = blockIdx.x % p.splits, cg = blockIdx.x / p.splits, kvh = blockIdx.y, b = blockIdx.z;
+  const Seq sq = sequence(p, b);
+  const int n_cols = sq.rows * p.group, col0 = cg * 16 * NT;
+  if (col0 >= n_cols) return;
+
+  bf16x8 qf[NT][HD / 32];
+  int lim[NT], most, least;
+  load_columns<HD, NT>(p, sq, b, kvh, col0, n_cols, lane, qf, lim, most, least);
   f32x4 acc[NT][VT];
   float m[NT], l[NT];
 #pragma unroll
@@ -212,7 +305,6 @@ __global__ __launch_bounds__(256) void attention_kernel(Params p) {
 
   const auto step = [&](Block<HD>& f, int block) {
     const int key0 = block * BLK;
-    const float ck = p.scale_log2 * kv8_pow2(f.ke - 127), ev = (float)(f.ve - 127), back = kv8_pow2(127 - f.ve);
     if (key0 + BLK > sq.len) {  // rows behind the last may hold anything
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -227,58 +319,9 @@ __global__ __launch_bounds__(256) void attention_kernel(Params p) {
 #pragma unroll
       for (int c = 0; c < HD / 32; ++c) a[t][c] = codes_bf16(f.k[t][c >> 1][2 * (c & 1)], f.k[t][c >> 1][2 * (c & 1) + 1]);
     f32x4 s[NT][2];
-#pragma unroll
-    for (int ct = 0; ct < NT; ++ct) scores<HD>(a, qf[ct], s[ct]);
-    float top[NT];
-    bool over = false;
-#pragma unroll
-    for (int ct = 0; ct < NT; ++ct) {
-      top[ct] = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[ct][t][i] = __builtin_fmaf(s[ct][t][i], ck, ev);
-      if (key0 + BLK > least) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (key0 + t * 16 + 4 * q + i >= lim[ct]) s[ct][t][i] = -INFINITY;
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top[ct] = fmaxf(top[ct], s[ct][t][i]);
-      over |= top[ct] > m[ct] + SLACK;
-    }
-    if (__any(over)) {
-#pragma unroll
-      for (int ct = 0; ct < NT; ++ct) {
-        const float now = fmaxf(m[ct], over_q_max(top[ct])), f0 = __builtin_amdgcn_exp2f(m[ct] - now);
-        m[ct] = now;
-        l[ct] *= f0;
-#pragma unroll
-        for (int t = 0; t < VT; ++t) acc[ct][t] *= f0;
-      }
-    }
+    scores<HD, 2, NT>(a, qf, s);
     f16x8 pf[NT];
-#pragma unroll
-    for (int ct = 0; ct < NT; ++ct) {
-      float sum = 0.f, e[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        e[j] = __builtin_amdgcn_exp2f(s[ct][j >> 2][j & 3] - m[ct]);
-        sum += e[j];
-      }
-      l[ct] = __builtin_fmaf(sum, back, l[ct]);
-      union {
-        f16x2 h[4];
-        f16x8 v;
-      } u;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) u.h[j] = __builtin_convertvector((md_f32pair{e[2 * j], e[2 * j + 1]}), f16x2);
-      pf[ct] = u.v;
-    }
+    softmax_block<NT, VT>(s, pf, acc, m, l, lim, key0 + BLK > least, key0, q, p.scale_log2 * kv8_pow2(f.ke - 127), (float)(f.ve - 127), kv8_pow2(127 - f.ve));
 #pragma unroll
     for (int c = 0; c < HD / 64; ++c) {
       const uint32_t w0[4] = {f.v[0][c], f.v[1][c], f.v[2][c], f.v[3][c]}, w1[4] = {f.v[4][c], f.v[5][c], f.v[6][c], f.v[7][c]};
@@ -295,103 +338,215 @@ __global__ __launch_bounds__(256) void attention_kernel(Params p) {
   };
 
   // two blocks' registers in turn: one on its way while the other is worked on (a block past the end is the last one again)
-  const int first = begin + (WK == 1 ? 0 : wave);
+  const int first = begin + wave;
   if (first < end) {
     Block<HD> f0, f1;
     load_block<HD>(f0, k, v, ke, ve, first, lane);
-    for (int block = first; block < end; block += 2 * WK) {
-      load_block<HD>(f1, k, v, ke, ve, min(block + WK, end - 1), lane);
+    for (int block = first; block < end; block += 8) {
+      load_block<HD>(f1, k, v, ke, ve, min(block + 4, end - 1), lane);
       step(f0, block);
-      load_block<HD>(f0, k, v, ke, ve, min(block + 2 * WK, end - 1), lane);
-      if (block + WK < end) step(f1, block + WK);
+      load_block<HD>(f0, k, v, ke, ve, min(block + 8, end - 1), lane);
+      if (block + 4 < end) step(f1, block + 4);
     }
   }
 #pragma unroll
   for (int ct = 0; ct < NT; ++ct) l[ct] = over_q_sum(l[ct]);
 
-  // a lane holds, of column r, coordinates VT (4 q + i) + t at acc[t][i]: VT * 4 neighbours
-  const int64_t bh = (int64_t)b * p.kv_heads + kvh;
-  if constexpr (WK == 1) {
+  // a lane holds, of column r, coordinates VT (4 q + i) + t at acc[t][i]
+  __shared__ float so[4][VT * 4][64];
+  __shared__ float sm[4][16], sl[4][16];
+  for (int ct = 0; ct < NT; ++ct) {
+    if (ct) __syncthreads();
 #pragma unroll
-    for (int ct = 0; ct < NT; ++ct) {
-      const int col = col0 + ct * 16 + r;
-      if (col >= n_cols) continue;
-      if (p.splits > 1) {
-        const int64_t at = (bh * p.cols + col) * p.splits + split;
-        float* out = p.part + at * HD + 4 * VT * q;
+    for (int t = 0; t < VT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int t = 0; t < VT; t += 4) *(f32x4*)(out + VT * i + t) = f32x4{acc[ct][t][i], acc[ct][t + 1][i], acc[ct][t + 2][i], acc[ct][t + 3][i]};
-        if (q == 0) {
-          p.part_ml[at * 2] = m[ct];
-          p.part_ml[at * 2 + 1] = l[ct];
-        }
-        continue;
-      }
-      const float inv = l[ct] == 0.f ? 0.f : 1.f / l[ct];
-      const int t0 = col / p.group, g = col - t0 * p.group;
-      bf16_t* out = p.o + (int64_t)b * p.o_bs + (int64_t)t0 * p.o_ts + (int64_t)(kvh * p.group + g) * p.o_hs + 4 * VT * q;
-      uint32_t w[2 * VT];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int t = 0; t < VT; t += 2) w[(VT * i + t) / 2] = pack_bf16x2(acc[ct][t][i] * inv, acc[ct][t + 1][i] * inv);
-#pragma unroll
-      for (int i = 0; i < VT / 2; ++i) *(u32x4*)(out + 8 * i) = u32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
-      if (p.lse && q == 0) p.lse[bh * p.cols + col] = l[ct] == 0.f ? INFINITY : m[ct] + __builtin_amdgcn_logf(l[ct]);
+      for (int i = 0; i < 4; ++i) so[wave][t * 4 + i][lane] = acc[ct][t][i];
+    if (q == 0) {
+      sm[wave][r] = m[ct];
+      sl[wave][r] = l[ct];
     }
+    __syncthreads();
+    float f[4], mm = NO_MAX, ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm[w][r]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      f[w] = __builtin_amdgcn_exp2f(sm[w][r] - mm);
+      ll = __builtin_fmaf(sl[w][r], f[w], ll);
+    }
+    const int col = col0 + ct * 16 + r;
+    if (col < n_cols) {  // wave i: coordinates VT (4 q + i) ..
+      float out[VT];
+#pragma unroll
+      for (int t = 0; t < VT; ++t) {
+        out[t] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) out[t] = __builtin_fmaf(so[w][t * 4 + wave][lane], f[w], out[t]);
+      }
+      store_column<HD, VT>(p, b, kvh, col, split, VT * (4 * q + wave), out, mm, ll, q == 0 && wave == 0);
+    }
+  }
+}
+
+// Many columns: every wave has its own NT tiles, and the four waves share the conversion: of the next two blocks, waves 0 and 1 bring the keys, 2 and 3
+// the values into LDS as the products' operands (16 bytes per lane, one operand after another: no bank conflicts either way), while all work on
+// the two before.  32 columns per wave: 48 and 64 need the registers of a third wave per SIMD, and larger workgroups even out worse over the CUs
+// (8 x 767 queries, 32 heads of 64: 61 us against 66 and 67; 2 x 2048 queries over 6101 rows, 32 on 8 heads of 128: 359 against 364 and 559).
+template <int HD, int NT>
+__global__ __launch_bounds__(256, 3) void prompt_kernel(Params p) {
+  constexpr int VT = HD / 16, KF = 2 * (HD / 32), W = HD / 64;
+  __shared__ u32x4 frag[2][2][KF + VT][64];  // [turn][block][operand][lane]
+  __shared__ float scale[2][2][2];           // [turn][block]: a key's exponent as a factor, a value's as a number
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  // Workgroup i runs on XCD i % 8.  Heads go to the XCDs in turn (a sequence's heads to all of them: sequences differ in length), and on an XCD the last
+  // queries, which see most, go first for all its heads.
+  const int per_head = p.splits * p.col_groups, heads = gridDim.x / per_head, full = heads / 8 * 8;
+  int id = blockIdx.x, head_id;
+  if (id < full * per_head) {
+    const int x = id & 7, n = full / 8;
+    id >>= 3;
+    head_id = id % n * 8 + x;
+    id /= n;
   } else {
-    static_assert(WK == 4 || WK == 1, "");
-    __shared__ float so[4][VT * 4][64];
-    __shared__ float sm[4][16], sl[4][16];
-    for (int ct = 0; ct < NT; ++ct) {
-      if (ct) __syncthreads();
+    id -= full * per_head;
+    head_id = full + id % (heads - full);
+    id /= heads - full;
+  }
+  const int split = id % p.splits, cg = p.col_groups - 1 - id / p.splits, kvh = head_id % p.kv_heads, b = head_id / p.kv_heads;
+  const Seq sq = sequence(p, b);
+  const int n_cols = sq.rows * p.group, wg0 = cg * 64 * NT, col0 = wg0 + wave * 16 * NT;
+  if (wg0 >= n_cols) return;
+
+  bf16x8 qf[NT][HD / 32];
+  int lim[NT], most, least;
+  load_columns<HD, NT>(p, sq, b, kvh, col0, n_cols, lane, qf, lim, most, least);
+  f32x4 acc[NT][VT];
+  float m[NT], l[NT];
 #pragma unroll
-      for (int t = 0; t < VT; ++t)
+  for (int ct = 0; ct < NT; ++ct) {
+    m[ct] = NO_MAX;
+    l[ct] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) so[wave][t * 4 + i][lane] = acc[ct][t][i];
-      if (q == 0) {
-        sm[wave][r] = m[ct];
-        sl[wave][r] = l[ct];
+    for (int t = 0; t < VT; ++t) acc[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // the workgroup's blocks: what its last query sees, or what the prefix does
+  const int first_pos = sq.pos0 + wg0 / p.group, last_pos = sq.pos0 + (min(n_cols, wg0 + 64 * NT) - 1) / p.group;
+  const int wg_most = max(limit_of(p, sq, first_pos), limit_of(p, sq, last_pos));
+  const int blocks = (wg_most + BLK - 1) / BLK, per = (blocks + p.splits - 1) / p.splits;
+  const int begin = split * per, end = min(begin + per, blocks);
+  const int64_t head = (int64_t)max(sq.slot, 0) * p.slot_stride + (int64_t)kvh * p.ctx * HD;
+  const int64_t ehead = (int64_t)max(sq.slot, 0) * p.exp_stride + (int64_t)kvh * (p.ctx / BLK);
+  const bool values = wave >= 2;
+  const int mine = wave & 1;  // of the two blocks
+  const uint8_t* codes = (values ? p.v : p.k) + head;
+  const uint8_t* exps = (values ? p.ve : p.ke) + ehead;
+
+  uint32_t st[8 * W];
+  int st_exp = 0;
+  const auto fetch = [&](int block0) {
+    const int block = min(block0 + mine, end - 1);
+    const uint8_t* at = codes + (int64_t)block * BLK * HD;
+    if (!values) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int c = 0; c < W; ++c) {
+          const u32x4 w = *(const u32x4*)(at + (t * 16 + r) * HD + c * 64 + q * 16);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) st[(t * W + c) * 4 + j] = w[j];
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint8_t* row = at + ((j < 4 ? 4 * q + j : 12 + 4 * q + j)) * HD + (HD / 16) * r;
+        if constexpr (HD == 64) {
+          st[j] = *(const uint32_t*)row;
+        } else {
+          const u32x2 w = *(const u32x2*)row;
+          st[2 * j] = w[0];
+          st[2 * j + 1] = w[1];
+        }
       }
-      __syncthreads();
-      float f[4], mm = NO_MAX, ll = 0.f;
+    }
+    st_exp = exps[block];
+  };
+  const auto convert = [&](int turn, int block0) {
+    if (!values) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm[w][r]);
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        f[w] = __builtin_amdgcn_exp2f(sm[w][r] - mm);
-        ll = __builtin_fmaf(sl[w][r], f[w], ll);
+        for (int c = 0; c < 2 * W; ++c)
+          frag[turn][mine][t * 2 * W + c][lane] = __builtin_bit_cast(u32x4, codes_bf16(st[t * 4 * W + 2 * c], st[t * 4 * W + 2 * c + 1]));
+      if (lane == 0) scale[turn][mine][0] = p.scale_log2 * kv8_pow2(st_exp - 127);
+    } else {
+      const int key0 = min(block0 + mine, end - 1) * BLK;
+      if (key0 + BLK > sq.len) {  // rows behind the last may hold anything
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (key0 + (j < 4 ? 4 * q + j : 12 + 4 * q + j) >= sq.len) {
+#pragma unroll
+            for (int c = 0; c < W; ++c) st[j * W + c] = 0;
+          }
       }
-      const int col = col0 + ct * 16 + r;
-      if (col < n_cols) {  // wave i: coordinates VT (4 q + i) ..
-        float out[VT];
+#pragma unroll
+      for (int c = 0; c < W; ++c) {
+        const uint32_t w0[4] = {st[c], st[W + c], st[2 * W + c], st[3 * W + c]}, w1[4] = {st[4 * W + c], st[5 * W + c], st[6 * W + c], st[7 * W + c]};
+        uint32_t t0[4], t1[4];
+        transpose4(w0, t0);
+        transpose4(w1, t1);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) frag[turn][mine][KF + 4 * c + t][lane] = __builtin_bit_cast(u32x4, codes_f16(t0[t], t1[t]));
+      }
+      if (lane == 0) scale[turn][mine][1] = (float)(st_exp - 127);
+    }
+  };
+
+  if (begin < end) {
+    fetch(begin);
+    convert(0, begin);
+    fetch(begin + 2);
+    __syncthreads();
+    int turn = 0;
+    for (int block0 = begin; block0 < end; block0 += 2, turn ^= 1) {
+      if (block0 + 2 < end) {
+        convert(turn ^ 1, block0 + 2);
+        fetch(block0 + 4);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key0 = (block0 + i) * BLK;
+        if (block0 + i >= end || key0 >= most) continue;  // (this wave's queries see none of it)
+        const float ck = scale[turn][i][0], ev = scale[turn][i][1];
+        bf16x8 a[2][HD / 32];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) a[t][c] = __builtin_bit_cast(bf16x8, frag[turn][i][t * (HD / 32) + c][lane]);
+        f32x4 s[NT][2];
+        scores<HD, 2, NT>(a, qf, s);
+        f16x8 pf[NT];
+        softmax_block<NT, VT>(s, pf, acc, m, l, lim, key0 + BLK > least, key0, q, ck, ev, __builtin_amdgcn_exp2f(-ev));
 #pragma unroll
         for (int t = 0; t < VT; ++t) {
-          out[t] = 0.f;
+          const f16x8 va = __builtin_bit_cast(f16x8, frag[turn][i][KF + t][lane]);
 #pragma unroll
-          for (int w = 0; w < 4; ++w) out[t] = __builtin_fmaf(so[w][t * 4 + wave][lane], f[w], out[t]);
-        }
-        const int at0 = VT * (4 * q + wave);
-        if (p.splits > 1) {
-          const int64_t at = (bh * p.cols + col) * p.splits + split;
-#pragma unroll
-          for (int t = 0; t < VT; t += 4) *(f32x4*)(p.part + at * HD + at0 + t) = f32x4{out[t], out[t + 1], out[t + 2], out[t + 3]};
-          if (q == 0 && wave == 0) {
-            p.part_ml[at * 2] = mm;
-            p.part_ml[at * 2 + 1] = ll;
-          }
-        } else {
-          const float inv = ll == 0.f ? 0.f : 1.f / ll;
-          const int t0 = col / p.group, g = col - t0 * p.group;
-          bf16_t* o = p.o + (int64_t)b * p.o_bs + (int64_t)t0 * p.o_ts + (int64_t)(kvh * p.group + g) * p.o_hs + at0;
-#pragma unroll
-          for (int t = 0; t < VT; t += 4) *(u32x2*)(o + t) = u32x2{pack_bf16x2(out[t] * inv, out[t + 1] * inv), pack_bf16x2(out[t + 2] * inv, out[t + 3] * inv)};
-          if (p.lse && q == 0 && wave == 0) p.lse[bh * p.cols + col] = ll == 0.f ? INFINITY : mm + __builtin_amdgcn_logf(ll);
+          for (int ct = 0; ct < NT; ++ct) acc[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[ct], acc[ct][t], 0, 0, 0);
         }
       }
+      __syncthreads();
     }
+  }
+#pragma unroll
+  for (int ct = 0; ct < NT; ++ct) {
+    l[ct] = over_q_sum(l[ct]);
+    const int col = col0 + ct * 16 + r;
+    if (col >= n_cols) continue;
+    float out[4 * VT];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < VT; ++t) out[VT * i + t] = acc[ct][t][i];
+    store_column<HD, 4 * VT>(p, b, kvh, col, split, 4 * VT * q, out, m[ct], l[ct], q == 0);
   }
 }
 
@@ -414,87 +569,145 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
     for (int i = 0; i < N; ++i) o[i] = __builtin_fmaf(part[(int64_t)s * HD + i], f, o[i]);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int t = col / p.group, g = col - t * p.group;
+  const int t = query_of(p, col), g = col - t * p.group;
   bf16_t* out = p.o + (int64_t)b * p.o_bs + (int64_t)t * p.o_ts + (int64_t)(kvh * p.group + g) * p.o_hs + lane * N;
 #pragma unroll
   for (int i = 0; i < N; ++i) out[i] = f2bf(o[i] * inv);
   if (p.lse && lane == 0) p.lse[c0] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
-// The weight that every row got: one wave per block of 32 rows, the block's keys in registers, all columns that see it pass by; scores are the ones of
-// the attention kernel again (the same products in the same order), exp2(score - lse) is their softmax.
+// The weight that every row got.  A wave holds 64 keys as operands; the columns that see them pass by, 64 at a time through LDS.  Of a workgroup's four
+// waves two have the same keys, one for each half of the columns (workgroups of 128 keys: more of them, for the sake of balance).  The
+// scores are the attention kernel's again (the same products in the same order), exp2(score - lse) is their softmax.
 template <int HD>
-__global__ __launch_bounds__(256) void weights_kernel(Params p) {
-  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, kvh = blockIdx.y, b = blockIdx.z;
-  const int block = blockIdx.x * 4 + (threadIdx.x >> 6), key0 = block * BLK;
+__global__ __launch_bounds__(256, 2) void weights_kernel(Params p) {
+  constexpr int KT = 4, QF = HD / 32, COLS = 64, PIECES = COLS / 16 * QF * 64 / 256;  // key tiles; operands of a column tile; 16-byte pieces per thread
+  __shared__ u32x4 frag[2][COLS / 16 * QF][64];
+  __shared__ float lses[2][COLS];
+  __shared__ int lims[2][COLS];
+  __shared__ float other[2][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4, kvh = blockIdx.y, b = blockIdx.z, half = wave & 1;
   const Seq sq = sequence(p, b);
-  if (key0 >= sq.len) return;
+  const int wg_key0 = blockIdx.x * 32 * KT, key0 = wg_key0 + (wave >> 1) * 16 * KT;
+  if (wg_key0 >= sq.len) return;
   const int64_t head = (int64_t)sq.slot * p.slot_stride + (int64_t)kvh * p.ctx * HD;
   const int64_t ehead = (int64_t)sq.slot * p.exp_stride + (int64_t)kvh * (p.ctx / BLK);
-  const uint8_t* kb = p.k + head + (int64_t)key0 * HD;
-  bf16x8 a[2][HD / 32];
+  bf16x8 a[KT][QF];
+  float ck[KT], w[KT][4] = {};
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int t = 0; t < KT; ++t) {
+    const int key = min(key0 + t * 16, p.ctx - 16);  // (what lies past the cache counts for nothing below)
+    ck[t] = p.scale_log2 * kv8_pow2((int)p.ke[ehead + key / BLK] - 127);
 #pragma unroll
     for (int c = 0; c < HD / 64; ++c) {
-      const u32x4 w = *(const u32x4*)(kb + (t * 16 + r) * HD + c * 64 + q * 16);
-      a[t][2 * c] = codes_bf16(w[0], w[1]);
-      a[t][2 * c + 1] = codes_bf16(w[2], w[3]);
+      const u32x4 x = *(const u32x4*)(p.k + head + (int64_t)(key + r) * HD + c * 64 + q * 16);
+      a[t][2 * c] = codes_bf16(x[0], x[1]);
+      a[t][2 * c + 1] = codes_bf16(x[2], x[3]);
     }
-  const float ck = p.scale_log2 * kv8_pow2((int)p.ke[ehead + block] - 127);
-  float w[2][4] = {};
+  }
   const float* lse = p.lse + ((int64_t)b * p.kv_heads + kvh) * p.cols;
   const int n_cols = sq.rows * p.group;
-  // queries from row key0 on see something of the block, those of the prefix if it begins within
-  const int t0 = key0 < p.prefix ? 0 : min(max(key0 - sq.pos0, 0), sq.rows);
-  for (int c0 = t0 * p.group; c0 < n_cols; c0 += 16) {
-    const int col = c0 + r;
-    bf16x8 qf[HD / 32];
-    load_query<HD>(p, b, kvh, col, sq.rows, q, qf);
-    const float ls = col < n_cols ? lse[col] : INFINITY;
-    const int lim = col < n_cols ? limit_of(p, sq, sq.pos0 + col / p.group) : 0;
-    f32x4 s[2];
-    scores<HD>(a, qf, s);
+  // queries from row wg_key0 on see something of these keys, those of the prefix if they begin within
+  const int begin = (wg_key0 < p.prefix ? 0 : min(max(wg_key0 - sq.pos0, 0), sq.rows)) * p.group;
+
+  u32x4 st[PIECES];
+  float st_lse = INFINITY;
+  int st_lim = 0;
+  const auto fetch = [&](int c0) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int i = 0; i < PIECES; ++i) {
+      const int f = i * 4 + wave, c = f % QF, col = min(c0 + f / QF * 16 + r, n_cols - 1), t = query_of(p, col), g = col - t * p.group;
+      st[i] = *(const u32x4*)(p.q + (int64_t)b * p.q_bs + (int64_t)t * p.q_ts + (int64_t)(kvh * p.group + g) * p.q_hs + (c >> 1) * 64 + q * 16 + (c & 1) * 8);
+    }
+    const int col = c0 + lane;  // (one that is none: it sees no key)
+    st_lse = lse[min(col, n_cols - 1)];
+    st_lim = col < n_cols ? limit_of(p, sq, sq.pos0 + query_of(p, col)) : 0;
+  };
+  const auto put = [&](int turn) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[t][i] += key0 + t * 16 + 4 * q + i < lim ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], ck, -ls)) : 0.f;
-  }
+    for (int i = 0; i < PIECES; ++i) frag[turn][i * 4 + wave][lane] = st[i] ^ u32x4{p.q_sign, p.q_sign, p.q_sign, p.q_sign};
+    if (wave == 0) {
+      lses[turn][lane] = st_lse;
+      lims[turn][lane] = st_lim;
+    }
+  };
+  if (begin < n_cols) {
+    fetch(begin);
+    put(0);
+    fetch(begin + COLS);
+    __syncthreads();
+    int turn = 0;
+    for (int c0 = begin; c0 < n_cols; c0 += COLS, turn ^= 1) {
+      if (c0 + COLS < n_cols) {
+        put(turn ^ 1);
+        fetch(c0 + 2 * COLS);
+      }
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+      for (int i = 0; i < 2; ++i) {
+        const int ct = half * 2 + i;
+        const float ls = lses[turn][ct * 16 + r];
+        const int lim = lims[turn][ct * 16 + r];
+        bf16x8 qf[1][QF];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int c = 0; c < QF; ++c) qf[0][c] = __builtin_bit_cast(bf16x8, frag[turn][ct * QF + c][lane]);
+        f32x4 sc[1][KT], (&s)[KT] = sc[0];
+        scores<HD, KT, 1>(a, qf, sc);
+        if (__any(lim < key0 + 16 * KT)) {
 #pragma unroll
-      for (int o = 1; o < 16; o <<= 1) w[t][i] += __shfl_xor(w[t][i], o, 64);
-  if (r < 8) {
-    const int t = r >> 2, i = r & 3, key = key0 + t * 16 + 4 * q + i;
-    float mine = 0.f;
+          for (int t = 0; t < KT; ++t)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) mine = j == r ? w[j >> 2][j & 3] : mine;
-    if (key < sq.len) {
-      float* out = p.weights + ((int64_t)sq.slot * p.kv_heads + kvh) * p.ctx + key;
-      *out = p.decay == 0.f ? mine : __builtin_fmaf(p.decay, *out, mine);
+            for (int j = 0; j < 4; ++j)
+              if (key0 + t * 16 + 4 * q + j >= lim) s[t][j] = -INFINITY;
+        }
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[t][j] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j], ck[t], -ls));
+      }
+      __syncthreads();
     }
   }
+  // over the 16 columns of a tile, then over the two halves; lane 4 t + j of a group of 16 has key 16 t + 4 q + j
+  float mine = 0.f;
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float x = w[t][j];
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o, 64);
+      mine = r == 4 * t + j ? x : mine;
+    }
+  if (half) other[wave >> 1][lane] = mine;
+  __syncthreads();
+  const int key = key0 + (r >> 2) * 16 + 4 * q + (r & 3);
+  if (!half && key < sq.len) {
+    mine += other[wave >> 1][lane];
+    float* out = p.weights + ((int64_t)sq.slot * p.kv_heads + kvh) * p.ctx + key;
+    *out = p.decay == 0.f ? mine : __builtin_fmaf(p.decay, *out, mine);
+  }
 }
+
+constexpr int PROMPT_NT = 2;
 
 // How a call is cut.  Up to 32 columns a wave's tiles would stand empty, and its keys are what there is to read: the four waves of a
 // workgroup share them.  Splits: enough workgroups for 256 CUs of 4 workgroups each, none with less than 8 blocks (decode) or 16.
 struct Plan {
-  int nt, wk, col_groups, splits, cols;
+  bool decode;
+  int nt, col_groups, splits, cols;
   size_t part, ml, lse, bytes;
 };
 
 Plan plan_of(const md_kv8_cache* c, const md_kv8_attn_args* a) {
   Plan pl;
   pl.cols = a->q_len * (a->n_heads / c->kv_heads);
-  pl.wk = pl.cols <= 32 ? 4 : 1;
-  pl.nt = pl.wk == 4 ? (pl.cols <= 16 ? 1 : 2) : (c->head_dim == 64 ? 4 : 2);
-  const int per = 16 * pl.nt * (4 / pl.wk);
+  pl.decode = pl.cols <= 32;
+  pl.nt = pl.decode ? (pl.cols <= 16 ? 1 : 2) : PROMPT_NT;
+  const int per = 16 * pl.nt * (pl.decode ? 1 : 4);
   pl.col_groups = (pl.cols + per - 1) / per;
   const int max_len = a->max_len > 0 ? std::min(a->max_len, c->ctx) : c->ctx, blocks = (max_len + BLK - 1) / BLK;
   const int64_t groups = (int64_t)pl.col_groups * c->kv_heads * a->batch;
-  const int64_t want = (1024 + groups - 1) / groups, most = std::max(1, blocks / (pl.wk == 4 ? 8 : 16));
+  const int64_t want = ((pl.decode ? 1024 : 512) + groups - 1) / groups, most = std::max(1, blocks / (pl.decode ? 8 : 16));
   pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 64}));
   const int64_t cols = (int64_t)a->batch * c->kv_heads * pl.cols;
   pl.part = 0;
@@ -507,7 +720,7 @@ Plan plan_of(const md_kv8_cache* c, const md_kv8_attn_args* a) {
 bool args_ok(const md_kv8_cache* c, const md_kv8_attn_args* a) {
   if (!kv8_cache_ok(c) || !a || a->batch <= 0 || a->q_len <= 0 || a->n_heads <= 0 || a->n_heads % c->kv_heads != 0 || a->max_len < 0) return false;
   const int64_t cols = (int64_t)a->q_len * (a->n_heads / c->kv_heads);
-  return cols <= 0x7fffff && a->batch <= 65535 && c->kv_heads <= 65535 && (a->slot || a->batch <= c->slots);
+  return cols <= 0x7fffff && cols * (a->n_heads / c->kv_heads) < (1ll << 32) && a->batch <= 65535 && c->kv_heads <= 65535 && (a->slot || a->batch <= c->slots);
 }
 
 }  // namespace
@@ -539,31 +752,38 @@ extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_at
   p.o_bs = a->o_bs, p.o_ts = a->o_ts, p.o_hs = a->o_hs;
   p.slot = a->slot, p.q_pos0 = a->q_pos0, p.q_rows = a->q_rows, p.kv_len = a->kv_len;
   p.group = a->n_heads / cache->kv_heads;
+  p.per_group = p.group > 1 ? (uint32_t)((1ull << 32) / p.group + 1) : 0;
+  p.all = p.group > 1 ? 0 : ~0u;
   p.q_len = a->q_len;
   p.max_len = a->max_len > 0 ? std::min(a->max_len, cache->ctx) : cache->ctx;
   p.prefix = a->prefix_len;
   p.splits = pl.splits, p.col_groups = pl.col_groups, p.cols = pl.cols;
-  p.scale_log2 = a->scale * LOG2E;
+  // (never 0: a masked score is -inf, and -inf * 0 is no number; 1e-25 times any score is as good)
+  p.scale_log2 = std::max(fabsf(a->scale) * LOG2E, 1e-25f);
+  p.q_sign = a->scale < 0.f ? 0x80008000u : 0u;
   p.decay = a->decay;
   char* ws = (char*)a->workspace;
   p.part = (float*)(ws + pl.part);
   p.part_ml = (float*)(ws + pl.ml);
   p.lse = a->weights ? (float*)(ws + pl.lse) : nullptr;
   p.weights = a->weights;
-  MD_CHECK_ARG((int64_t)pl.col_groups * pl.splits <= 0x7fffffff);
-  const dim3 grid(pl.col_groups * pl.splits, cache->kv_heads, a->batch), block(256);
+  const int64_t groups = (int64_t)pl.col_groups * pl.splits, all = groups * cache->kv_heads * a->batch;
+  MD_CHECK_ARG(all <= 0x7fffffff);
+  const dim3 grid(groups, cache->kv_heads, a->batch), block(256);
   hipStream_t s = (hipStream_t)stream;
-#define MD_ATTN(HD, NT, WK) hipLaunchKernelGGL((attention_kernel<HD, NT, WK>), grid, block, 0, s, p)
-  if (cache->head_dim == 64) {
-    if (pl.wk == 1) MD_ATTN(64, 4, 1);
-    else if (pl.nt == 1) MD_ATTN(64, 1, 4);
-    else MD_ATTN(64, 2, 4);
+  if (pl.decode) {
+    if (cache->head_dim == 64) {
+      if (pl.nt == 1) hipLaunchKernelGGL((decode_kernel<64, 1>), grid, block, 0, s, p);
+      else hipLaunchKernelGGL((decode_kernel<64, 2>), grid, block, 0, s, p);
+    } else {
+      if (pl.nt == 1) hipLaunchKernelGGL((decode_kernel<128, 1>), grid, block, 0, s, p);
+      else hipLaunchKernelGGL((decode_kernel<128, 2>), grid, block, 0, s, p);
+    }
+  } else if (cache->head_dim == 64) {
+    hipLaunchKernelGGL((prompt_kernel<64, PROMPT_NT>), dim3(all), block, 0, s, p);
   } else {
-    if (pl.wk == 1) MD_ATTN(128, 2, 1);
-    else if (pl.nt == 1) MD_ATTN(128, 1, 4);
-    else MD_ATTN(128, 2, 4);
+    hipLaunchKernelGGL((prompt_kernel<128, PROMPT_NT>), dim3(all), block, 0, s, p);
   }
-#undef MD_ATTN
   MD_TRY(md_launch_status());
   if (pl.splits > 1) {
     const dim3 jg((pl.cols + 3) / 4, cache->kv_heads, a->batch);
@@ -572,7 +792,7 @@ extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_at
     MD_TRY(md_launch_status());
   }
   if (a->weights) {
-    const dim3 wg((((p.max_len + BLK - 1) / BLK) + 3) / 4, cache->kv_heads, a->batch);
+    const dim3 wg((p.max_len + 127) / 128, cache->kv_heads, a->batch);
     if (cache->head_dim == 64) hipLaunchKernelGGL(weights_kernel<64>, wg, block, 0, s, p);
     else hipLaunchKernelGGL(weights_kernel<128>, wg, block, 0, s, p);
     MD_TRY(md_launch_status());

@@ -3,11 +3,12 @@
 //   total(k, t) = score_k + logit_t - log sum_v exp(logit_v)
 // Within a beam totals follow the logits, so a beam's candidates are its `beams` largest logits (ties: the lower token): one pass over the
 // logits gives them and the sum, and only beams x beams totals are ever compared.
-//   part_kernel    one workgroup per (beam, piece of the vocabulary): the piece in registers; each wave's largest logits one after another
-//                  (only the lane that gave one looks for its next), its maximum and its sum of exponentials
-//   choose_kernel  one workgroup per input: sums joined in 64 bits, every beam's candidates, totals, their order by counting who is ahead
+//   part_kernel    one workgroup per (beam, piece of the vocabulary): the piece in registers; each wave's largest logits, its maximum and its sum
+//                  of exponentials
+//   choose_kernel  one workgroup per input, one wave per beam: sums joined in 64 bits, the beam's candidates; totals, their order by counting
+//                  who is ahead
 // Bound by the logits' bytes; with few rows by the two launches.
-#include "md_common.hpp"
+#include "wave_ops.hpp"
 
 #include <algorithm>
 
@@ -16,6 +17,7 @@ namespace {
 constexpr int PIECE = 8192;  // logits of a workgroup: 32 per thread
 constexpr int PER = PIECE / 256;
 constexpr int MAXB = MD_MAX_BEAMS;
+constexpr int ROOM = 128;    // logits of a wave that are put in order together
 constexpr float F32_MOST = 3.4028234663852886e38f;
 
 // (value, index) as one number: the larger value first, of equal ones the lower index.  0 stands for nothing.
@@ -30,13 +32,10 @@ __device__ __forceinline__ float value_of(uint64_t c) {
 }
 __device__ __forceinline__ uint32_t index_of(uint64_t c) { return ~(uint32_t)c; }
 
-__device__ __forceinline__ uint64_t wave_most(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint64_t w = __shfl_xor((unsigned long long)v, o, 64);
-    v = w > v ? w : v;
-  }
-  return v;
+// exp(x), x <= 0, to an ulp or two of fp32: what the product x * log2(e) lost goes into the result
+__device__ __forceinline__ float exp_of(float x) {
+  const float a = x * 1.44269502f, lost = __builtin_fmaf(x, 1.44269502f, -a) + x * 1.92596299e-8f, e = __builtin_amdgcn_exp2f(a);
+  return a > -126.f ? __builtin_fmaf(e, lost * 0.693147182f, e) : 0.f;
 }
 
 // a beam that has continuations of its own
@@ -56,11 +55,13 @@ __global__ __launch_bounds__(256) void part_kernel(const T* __restrict__ logits,
                                                    const float* __restrict__ scores, const int32_t* __restrict__ ended, int pieces,
                                                    uint64_t* __restrict__ best, double* __restrict__ sums) {
   constexpr int E = 16 / sizeof(T), N = PER / E;  // elements of a load, loads of a thread
-  __shared__ uint64_t lists[4 * MAXB];
+  __shared__ uint64_t lists[4 * MAXB], found[4][ROOM];
   __shared__ float wmax[4];
   __shared__ double wsum[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, piece = blockIdx.x, row = blockIdx.y;
   if (!goes_on(scores, ended, row)) return;
+  if (threadIdx.x < 8) lists[min(4 * beams + (int)threadIdx.x, 4 * MAXB - 1)] = 0;  // (the count runs over whole eights)
+  __syncthreads();
   const T* x = logits + (int64_t)row * ld;
   const int base = piece * PIECE;
   const bool aligned = ((uintptr_t)x & 15) == 0;
@@ -78,38 +79,80 @@ __global__ __launch_bounds__(256) void part_kernel(const T* __restrict__ logits,
       for (int j = 0; j < E; ++j) v[i * E + j] = at + j < vocab ? logit<T>(x[at + j]) : -INFINITY;
     }
   }
+  const auto id_of = [&](int i) { return base + ((i / E) * 256 + (int)threadIdx.x) * E + i % E; };
+  if ((unsigned)(suppress_id - base) < (unsigned)PIECE) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = id_of(i) == suppress_id ? -INFINITY : v[i];
+  }
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int id = base + ((i / E) * 256 + (int)threadIdx.x) * E + i % E;
-    v[i] = v[i] == v[i] && id != suppress_id ? fminf(v[i], F32_MOST) : -INFINITY;
+    v[i] = v[i] == v[i] ? fminf(v[i], F32_MOST) : -INFINITY;
     top = fmaxf(top, v[i]);
   }
-  const float m = wave_max(top);
+  const float m = wave_most_f32(top);
   double sum = 0.;
   if (m > -INFINITY) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sum += (double)expf(v[i] - m);
-  }
+    for (int i = 0; i < PER; i += 4) {
+      float s4 = 0.f;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-
-  uint64_t taken = ~0ull, mine = 0;
-  const auto next = [&]() {  // this thread's largest below what it gave last
-    mine = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const uint64_t c = candidate(v[i], base + ((i / E) * 256 + (int)threadIdx.x) * E + i % E);
-      if (v[i] > -INFINITY && c < taken && c > mine) mine = c;
+      for (int j = 0; j < 4; ++j) s4 += exp_of(v[i + j] - m);
+      sum += (double)s4;
     }
-  };
-  next();
-  for (int k = 0; k < beams; ++k) {
-    const uint64_t c = wave_most(mine);
-    if (lane == 0) lists[wave * beams + k] = c;
-    if (c != 0 && c == mine) {
-      taken = c;
-      next();
+  }
+  sum = wave_sum_f64(sum);
+
+  // The wave's `beams` largest: at least as many logits reach the beams-th largest of the lanes' maxima, and seldom many more; those that do are
+  // collected and put in order by counting.  Where very many do (equal logits), one after another is looked for.
+  int above = 0;
+#pragma unroll
+  for (int j = 0; j < 64; ++j) above += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(top), j)) > top ? 1 : 0;
+  const float least = -wave_most_f32(above < beams ? -top : -INFINITY);  // (of equal maxima all count as the first)
+  int mine_n = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) mine_n += v[i] >= least && v[i] > -INFINITY ? 1 : 0;
+  const uint32_t upto = wave_scan_u32((uint32_t)mine_n);
+  const int n = (int)lane_63(upto);
+  if (mine_n) {
+    int place = (int)upto - mine_n;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (v[i] >= least && v[i] > -INFINITY) {
+        if (place < ROOM) found[wave][place] = candidate(v[i], id_of(i));
+        ++place;
+      }
+  }
+  if (n <= ROOM) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (a wave's LDS accesses run in order)
+    if (lane < beams) lists[wave * beams + lane] = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int i = lane; i < n; i += 64) {
+      const uint64_t c = found[wave][i];
+      int ahead = 0;
+      for (int j = 0; j < n; j += 8)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) ahead += found[wave][j + u] > c && j + u < n;  // (ROOM % 8 == 0)
+      if (ahead < beams) lists[wave * beams + ahead] = c;
+    }
+  } else {
+    uint64_t taken = ~0ull, mine = 0;
+    const auto next = [&]() {  // this thread's largest below what it gave last
+      mine = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const uint64_t c = candidate(v[i], id_of(i));
+        if (v[i] > -INFINITY && c < taken && c > mine) mine = c;
+      }
+    };
+    next();
+    for (int k = 0; k < beams; ++k) {
+      const uint64_t c = wave_most_u64(mine);
+      if (lane == 0) lists[wave * beams + k] = c;
+      if (c != 0 && c == mine) {
+        taken = c;
+        next();
+      }
     }
   }
   if (lane == 0) {
@@ -118,10 +161,12 @@ __global__ __launch_bounds__(256) void part_kernel(const T* __restrict__ logits,
   }
   __syncthreads();
   if (wave == 0) {  // of at most 64 the largest, one per lane, each at the place that counting gives it
-    const int n = 4 * beams;
+    const int n = (4 * beams + 7) & ~7;
     const uint64_t c = lane < n ? lists[lane] : 0;
     int ahead = 0;
-    for (int j = 0; j < n; ++j) ahead += lists[j] > c || (lists[j] == c && j < lane);
+    for (int j = 0; j < n; j += 8)  // (n % 8 == 0)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) ahead += lists[j + u] > c || (lists[j + u] == c && j + u < lane);
     if (lane < n && ahead < beams) best[((int64_t)row * pieces + piece) * beams + ahead] = c;
     if (lane == 0) {
       const float mm = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
@@ -139,73 +184,90 @@ struct Ranked {
   uint64_t logit;  // candidate(): the logit and its token
 };
 
-__global__ __launch_bounds__(256) void choose_kernel(int beams, int pieces, int end_id, const float* scores, const int32_t* ended,
-                                                     const float* __restrict__ rank_weight, const uint64_t* __restrict__ best,
-                                                     const double* __restrict__ sums, int32_t* __restrict__ tokens, int32_t* __restrict__ parents,
-                                                     float* scores_out, int32_t* ended_out) {
+__global__ __launch_bounds__(64 * MAXB) void choose_kernel(int beams, int pieces, int end_id, const float* scores, const int32_t* ended,
+                                                           const float* __restrict__ rank_weight, const uint64_t* __restrict__ best,
+                                                           const double* __restrict__ sums, int32_t* __restrict__ tokens, int32_t* __restrict__ parents,
+                                                           float* scores_out, int32_t* ended_out) {
   __shared__ Ranked cand[MAXB * MAXB];
   __shared__ double totals[MAXB * MAXB];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.x, row0 = b * beams, n = beams * beams;
-  for (int k = wave; k < beams; k += 4) {
-    const int row = row0 + k;
-    const float score = scores[row], weight = rank_weight ? rank_weight[row] : 1.f;
-    if (!goes_on(scores, ended, row)) {  // (an ended beam of a score: itself, and nothing else)
-      if (lane < beams) {
-        const bool itself = lane == 0 && score > -INFINITY;
-        cand[k * beams + lane] = {itself ? (double)score * (double)weight : -INFINITY, itself ? candidate(0.f, end_id) : 0};
-        totals[k * beams + lane] = itself ? (double)score : -INFINITY;
-      }
-      continue;
+  __shared__ int counts[MAXB * MAXB + 1];  // of every candidate who is ahead; candidates
+  if ((int)threadIdx.x <= MAXB * MAXB) {
+    for (int i = threadIdx.x; i <= MAXB * MAXB; i += blockDim.x) counts[i] = 0;
+  }
+  const int lane = threadIdx.x & 63, k = threadIdx.x >> 6, b = blockIdx.x, row0 = b * beams, n = beams * beams, row = row0 + k;
+  const float score = scores[row], weight = rank_weight ? rank_weight[row] : 1.f;
+  if (!goes_on(scores, ended, row)) {  // (an ended beam of a score: itself, and nothing else)
+    if (lane < beams) {
+      const bool itself = lane == 0 && score > -INFINITY;
+      cand[k * beams + lane] = {itself ? (double)score * (double)weight : -INFINITY, itself ? candidate(0.f, end_id) : 0};
+      totals[k * beams + lane] = itself ? (double)score : -INFINITY;
     }
-    double m = -INFINITY, s = 0.;
-    for (int i = 0; i < pieces; ++i) m = fmax(m, sums[((int64_t)row * pieces + i) * 2]);
-    for (int i = lane; i < pieces; i += 64) {
-      const double pm = sums[((int64_t)row * pieces + i) * 2];
-      if (pm > -INFINITY) s += sums[((int64_t)row * pieces + i) * 2 + 1] * exp(pm - m);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    const double norm = m + log(s);
+  } else {
     const uint64_t* list = best + (int64_t)row * pieces * beams;
-    uint64_t taken = ~0ull;
-    for (int j = 0; j < beams; ++j) {
-      uint64_t c = 0;
-      for (int i = lane; i < pieces * beams; i += 64) {
-        const uint64_t e = list[i];
-        if (e < taken && e > c) c = e;
+    uint64_t carry = 0;  // carry: lane j has the j-th largest so far
+    double m = -INFINITY, s = 0.;
+    for (int i = 0; i < pieces; i += 64) {
+      const bool in = i + lane < pieces;
+      const double pm = in ? sums[((int64_t)row * pieces + i + lane) * 2] : -INFINITY, ps = in ? sums[((int64_t)row * pieces + i + lane) * 2 + 1] : 0.;
+      const double now = fmax(m, (double)wave_most_f32((float)pm));  // (maxima of logits: exact in fp32)
+      if (now > -INFINITY) {
+        s = (m > -INFINITY ? s * exp(m - now) : 0.) + (pm > -INFINITY ? ps * exp(pm - now) : 0.);  // (this lane's share)
+        m = now;
       }
-      c = wave_most(c);
-      taken = c;
-      if (lane == 0) {
-        const double total = c ? (double)score + ((double)value_of(c) - norm) : -INFINITY;
-        const bool real = total > -INFINITY;
-        cand[k * beams + j] = {real ? total * (double)weight : -INFINITY, real ? c : 0};
-        totals[k * beams + j] = real ? total : -INFINITY;
+    }
+    s = wave_sum_f64(s);
+    const double norm = m + log(s);
+    // A piece's list is in falling order: lane i goes along piece i's, its next entry on its way.  (More than 64 pieces: 64 at a time, the largest so far
+    // as one more entry of each lane.)
+    for (int first = 0; first < pieces; first += 64) {
+      const int piece = first + lane;
+      const uint64_t* mine = list + (int64_t)min(piece, pieces - 1) * beams;
+      uint64_t head = piece < pieces ? mine[0] : 0, next = piece < pieces ? mine[1] : 0, got = 0;
+      int at = 1;
+      for (int j = 0; j < beams; ++j) {
+        const uint64_t w = wave_most_u64(head > carry ? head : carry);
+        if (lane == j) got = w;
+        if (carry == w) carry = 0;
+        if (head == w && w != 0) {
+          head = next;
+          ++at;
+          next = at < beams ? mine[at] : 0;
+        }
       }
+      carry = got;
+    }
+    if (lane < beams) {
+      const double total = carry ? (double)score + ((double)value_of(carry) - norm) : -INFINITY;
+      const bool real = total > -INFINITY;
+      cand[k * beams + lane] = {real ? total * (double)weight : -INFINITY, real ? carry : 0};
+      totals[k * beams + lane] = real ? total : -INFINITY;
     }
   }
   __syncthreads();
   // (every input of this input's beams has been read: what follows may overwrite scores and ended)
-  const int i = threadIdx.x;
-  const Ranked me = i < n ? cand[i] : Ranked{-INFINITY, 0};
-  const int parent = i / beams;
-  int was_ended = 0;
-  if (i < n) was_ended = ended && ended[row0 + parent] != 0;
-  int live = 0, ahead = 0;
-  for (int j = 0; j < n; ++j) {
+  // thread (i, part): who of `part`'s share of the candidates is ahead of candidate i
+  const int parts = 64 / beams, i = (int)threadIdx.x % n, part = (int)threadIdx.x / n, parent = i / beams;
+  const Ranked me = cand[i];
+  const int was_ended = ended && ended[row0 + parent] != 0;
+  int ahead = 0;
+  for (int j = part; part < parts && j < n; j += parts) {
+    const int p = (j * (65536 / beams + 1)) >> 16;  // j / beams
     const Ranked o = cand[j];
-    live += o.logit != 0;
-    ahead += o.logit != 0 && (o.rank > me.rank || (o.rank == me.rank && (j / beams < parent || (j / beams == parent && o.logit > me.logit))));
+    ahead += o.logit != 0 && (o.rank > me.rank || (o.rank == me.rank && (p < parent || (p == parent && o.logit > me.logit))));
   }
+  if (ahead) atomicAdd(&counts[i], ahead);
+  if (part == 0 && me.logit != 0) atomicAdd(&counts[MAXB * MAXB], 1);
   __syncthreads();
-  if (i < n && me.logit != 0 && ahead < beams) {
+  ahead = counts[i];
+  const int live = counts[MAXB * MAXB];
+  if (part == 0 && me.logit != 0 && ahead < beams) {
     const int token = (int)index_of(me.logit), at = row0 + ahead;
     tokens[at] = token;
     parents[at] = parent;
     scores_out[at] = (float)totals[i];
     if (ended_out) ended_out[at] = was_ended || token == end_id;
   }
-  if (i < beams && i >= live) {
+  if (part == 0 && i < beams && i >= live) {
     tokens[row0 + i] = end_id;
     parents[row0 + i] = i;
     scores_out[row0 + i] = -INFINITY;
@@ -232,7 +294,7 @@ struct Parts {
 };
 
 template <typename W, int B>
-__device__ __forceinline__ void move_words(const Part& p, int64_t first, const int32_t* par, int beams, int64_t slot0) {
+__device__ __forceinline__ void move_words(const Part& p, int64_t first, const int32_t* __restrict__ parents, int beams, int64_t slot0) {
   const int64_t w = first + threadIdx.x;
   if (w >= p.words) return;
   const int64_t run = w / p.per_seg;
@@ -243,31 +305,30 @@ __device__ __forceinline__ void move_words(const Part& p, int64_t first, const i
   const bool in_place = p.src == p.dst;
   W v[B];
 #pragma unroll
-  for (int i = 0; i < B; ++i)
-    if (i < beams && !(in_place && par[i] == i)) v[i] = *(const W*)(src + par[i] * p.src_slot);
+  for (int i = 0; i < B; ++i) {
+    if (i >= beams) continue;
+    const int q = parents[i], from = q >= 0 && q < beams ? q : i;
+    if (!in_place || from != i) v[i] = *(const W*)(src + from * p.src_slot);
+  }
 #pragma unroll
-  for (int i = 0; i < B; ++i)
-    if (i < beams && !(in_place && par[i] == i)) *(W*)(dst + i * p.dst_slot) = v[i];
+  for (int i = 0; i < B; ++i) {
+    if (i >= beams) continue;
+    const int q = parents[i], from = q >= 0 && q < beams ? q : i;
+    if (!in_place || from != i) *(W*)(dst + i * p.dst_slot) = v[i];
+  }
 }
 
 // One thread per word of a slot, for all beams of an input: every word is read from all parents before it is written to any child, so in place
 // needs no second copy and no order among workgroups.
 template <int B>
 __global__ __launch_bounds__(256) void reorder_kernel(Parts parts, const int32_t* __restrict__ parents, int beams) {
-  __shared__ int32_t par[B];
   int i = 0;
   while (i + 1 < parts.n && (int)blockIdx.x >= parts.p[i + 1].first) ++i;
   const Part& p = parts.p[i];
-  const int b = blockIdx.y;
-  if ((int)threadIdx.x < beams) {
-    const int q = parents[(int64_t)b * beams + threadIdx.x];
-    par[threadIdx.x] = q >= 0 && q < beams ? q : threadIdx.x;
-  }
-  __syncthreads();
-  const int64_t first = (int64_t)((int)blockIdx.x - p.first) * 256;
-  if (p.width == 16) move_words<u32x4, B>(p, first, par, beams, (int64_t)b * beams);
-  else if (p.width == 4) move_words<uint32_t, B>(p, first, par, beams, (int64_t)b * beams);
-  else move_words<uint8_t, B>(p, first, par, beams, (int64_t)b * beams);
+  const int64_t slot0 = (int64_t)blockIdx.y * beams, first = (int64_t)((int)blockIdx.x - p.first) * 256;
+  if (p.width == 16) move_words<u32x4, B>(p, first, parents + slot0, beams, slot0);
+  else if (p.width == 4) move_words<uint32_t, B>(p, first, parents + slot0, beams, slot0);
+  else move_words<uint8_t, B>(p, first, parents + slot0, beams, slot0);
 }
 
 int64_t extent(const md_state_part& s, bool src, int64_t slots) {
@@ -311,7 +372,7 @@ extern "C" md_status md_beam_select(const md_beam_args* a, void* stream) {
   else
     hipLaunchKernelGGL(part_kernel<float>, grid, dim3(256), 0, s, (const float*)a->logits, a->ld, a->vocab, a->beams, a->suppress_id, a->scores, a->ended,
                        pieces, best, sums);
-  hipLaunchKernelGGL(choose_kernel, dim3(a->batch), dim3(256), 0, s, a->beams, pieces, a->end_id, a->scores, a->ended, a->rank_weight, best, sums,
+  hipLaunchKernelGGL(choose_kernel, dim3(a->batch), dim3(64 * a->beams), 0, s, a->beams, pieces, a->end_id, a->scores, a->ended, a->rank_weight, best, sums,
                      a->tokens, a->parents, a->scores_out, a->ended_out);
   return md_launch_status();
 }
@@ -338,7 +399,6 @@ extern "C" md_status md_state_reorder(const md_state_part* parts, int32_t n_part
     const dim3 grid((unsigned)groups, batch);
     hipStream_t st = (hipStream_t)stream;
     if (beams <= 4) hipLaunchKernelGGL(reorder_kernel<4>, grid, dim3(256), 0, st, ps, parents, beams);
-    else if (beams <= 8) hipLaunchKernelGGL(reorder_kernel<8>, grid, dim3(256), 0, st, ps, parents, beams);
     else hipLaunchKernelGGL(reorder_kernel<16>, grid, dim3(256), 0, st, ps, parents, beams);
     MD_TRY(md_launch_status());
   }

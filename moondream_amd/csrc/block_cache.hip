@@ -4,6 +4,7 @@
 // or 16 (evict) neighbouring coordinates of a few rows, and any lane may hold any row, because the block has ONE scale; so every
 // memory instruction of the wave covers whole rows, one after another.  All three are bound by memory.
 #include "block_cache.hpp"
+#include "wave_ops.hpp"
 
 #include <algorithm>
 
@@ -49,6 +50,7 @@ __global__ __launch_bounds__(256) void append_kernel(Cache c, Rows k, Rows v, co
   const bf16_t* x = in.x + (int64_t)b * in.bs + (int64_t)h * in.hs;
   uint8_t* codes = (which ? c.v : c.k) + (int64_t)sl * c.slot_stride + ((int64_t)h * c.ctx + base) * HD;
   uint8_t* ep = (which ? c.ve : c.ke) + (int64_t)sl * c.exp_stride + (int64_t)h * (c.ctx / BLK) + block;
+  const int was = *ep;
   u32x4 q[N];
   float top = 0.f;
 #pragma unroll
@@ -61,9 +63,9 @@ __global__ __launch_bounds__(256) void append_kernel(Cache c, Rows k, Rows v, co
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int w = 0; w < 4; ++w) top = fmaxf(top, fmaxf(kv8_magnitude(lo_bf(q[i][w])), kv8_magnitude(hi_bf(q[i][w]))));
-  int e = kv8_exponent(wave_max(top));
+  int e = kv8_exponent(wave_most_f32(top));
   if (base < r0) {  // older rows: their scale stays, or they are rounded to the larger one
-    const int old = min(max((int)*ep - 127, MD_KV8_MIN_EXP), MD_KV8_MAX_EXP);
+    const int old = min(max(was - 127, MD_KV8_MIN_EXP), MD_KV8_MAX_EXP);
     if (e <= old) {
       e = old;
     } else {
@@ -147,12 +149,7 @@ constexpr int DIGIT = 11;   // bits of a key that one pass decides: three passes
 // sums over the threads before this one, and of all; `part` has 16 places
 __device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* part, uint32_t& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t s = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t t = __shfl_up(s, o, 64);
-    if (lane >= o) s += t;
-  }
+  const uint32_t s = wave_scan_u32(v);
   if (lane == 63) part[wave] = s;
   __syncthreads();
   uint32_t before = 0, all = 0;
@@ -168,14 +165,19 @@ __device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* part, uint
 }
 
 // One workgroup per (head, sequence): the keep-th largest key digit by digit (a histogram in LDS each), then the rows in their order: those above
-// it, and as many of its equals, lowest first, as are still wanted.
+// it, and as many of its equals, lowest first, as are still wanted.  Up to HELD * 1024 rows are read once and stay in registers, longer caches
+// come by portion by portion in every pass.  Of a portion a wave has HELD * 64 rows in a row, of these a lane four in a row, 256 apart.  COPIES of the
+// histogram lie in different banks, so that lanes that count the same digit (the first digit is sign, exponent and two bits: few are in use) mostly
+// do so in different places.  Caches of up to 4096 rows take HELD 4, COPIES 2: 801 rows of 32 heads in 8 us against 25 with 32 and 8.
+template <int HELD, int COPIES>
 __global__ __launch_bounds__(SEL) void select_kernel(const float* __restrict__ weights, const int32_t* __restrict__ slot,
                                                      const int32_t* __restrict__ kv_len, int32_t* __restrict__ kept, int slots, int ctx, int heads, int keep,
                                                      int first, int recent) {
-  __shared__ uint32_t hist[1 << DIGIT];
+  constexpr int APART = (1 << DIGIT) + 4;
+  __shared__ uint32_t hist[APART * COPIES];
   __shared__ uint32_t part[SEL / 64];
   __shared__ uint32_t found[2];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int32_t* out = kept + ((int64_t)b * heads + h) * keep;
   const int sl = slot ? slot[b] : b;
   const int len = sl < 0 || sl >= slots ? 0 : min(max(kv_len[b], 0), ctx);
@@ -184,18 +186,46 @@ __global__ __launch_bounds__(SEL) void select_kernel(const float* __restrict__ w
     return;
   }
   const float* w = weights + ((int64_t)sl * heads + h) * ctx;
+  const bool quads = ((uintptr_t)w & 15) == 0;  // (ctx % 32 == 0: all heads' or none's)
+  uint32_t key[HELD];
+  const auto load = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < HELD; i += 4) {
+      const int j = j0 + wave * (HELD * 64) + i * 64 + lane * 4;
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      if (j + 3 < ctx && quads) {
+        x = *(const f32x4*)(w + j);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j + e < ctx) x[e] = w[j + e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) key[i + e] = rank_key(x[e], j + e < first || j + e >= len - recent);
+    }
+  };
+  const auto row_of = [&](int j0, int i) { return j0 + wave * (HELD * 64) + (i & ~3) * 64 + lane * 4 + (i & 3); };
+  const bool one = len <= HELD * SEL;
+  if (one) load(0);
   uint32_t prefix = 0, mask = 0, want = keep;  // the key's leading digits, and how many of those that share them stay
-  for (int shift = 32 - DIGIT; ; shift = max(shift - DIGIT, 0)) {
-    for (int j = tid; j < (1 << DIGIT); j += SEL) hist[j] = 0;
+  for (int shift = 32 - DIGIT;; shift = max(shift - DIGIT, 0)) {
+    for (int j = tid; j < APART * COPIES; j += SEL) hist[j] = 0;
     __syncthreads();
-    for (int j = tid; j < len; j += SEL) {
-      const uint32_t key = rank_key(w[j], j < first || j >= len - recent);
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & ((1 << DIGIT) - 1)], 1u);
+    for (int j0 = 0; j0 < len; j0 += HELD * SEL) {
+      if (!one) load(j0);
+#pragma unroll
+      for (int i = 0; i < HELD; ++i)
+        if (row_of(j0, i) < len && (key[i] & mask) == prefix) atomicAdd(&hist[((key[i] >> shift) & ((1 << DIGIT) - 1)) + (lane & (COPIES - 1)) * APART], 1u);
     }
     __syncthreads();
     // this thread's two digits, the larger first: how many keys lie above them
     const int d1 = (1 << DIGIT) - 1 - 2 * tid, d0 = d1 - 1;
-    const uint32_t n1 = hist[d1], n0 = hist[d0];
+    uint32_t n1 = 0, n0 = 0;
+#pragma unroll
+    for (int c = 0; c < COPIES; ++c) {
+      n1 += hist[d1 + c * APART];
+      n0 += hist[d0 + c * APART];
+    }
     uint32_t total;
     const uint32_t above = scan_before(n1 + n0, part, total);
     if (above < want && above + n1 >= want) {
@@ -214,16 +244,38 @@ __global__ __launch_bounds__(SEL) void select_kernel(const float* __restrict__ w
   }
   // `prefix` is the key, `want` of its equals stay.  (The last pass's digit overlaps the one before by a bit, which is then settled.)
   uint32_t n_above = 0, n_equal = 0;
-  for (int j0 = 0; j0 < len; j0 += SEL) {
-    const int j = j0 + tid;
-    const uint32_t key = j < len ? rank_key(w[j], j < first || j >= len - recent) : 0;
-    const bool above = j < len && key > prefix, equal = j < len && key == prefix;
-    uint32_t total;
-    const uint32_t before = scan_before((above ? 1u : 0u) + (equal ? 1u << 16 : 0u), part, total);
-    const uint32_t eq = n_equal + (before >> 16), at = n_above + (before & 0xffffu) + min(eq, want);
-    if (above || (equal && eq < want)) out[at] = j;
-    n_above += total & 0xffffu;
-    n_equal += total >> 16;
+  for (int j0 = 0; j0 < len; j0 += HELD * SEL) {
+    if (!one) load(j0);
+    // above in the low half, equal in the high one: 32768 at most
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+      if (row_of(j0, i) < len) mine += (key[i] > prefix ? 1u : 0u) + (key[i] == prefix ? 1u << 16 : 0u);
+    uint32_t all, before = scan_before(mine, part, all);
+    before = __builtin_amdgcn_readfirstlane(before);  // of the wave's first lane: all earlier waves'
+    for (int i = 0; i < HELD; i += 4) {
+      uint32_t quad[4], sum = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        quad[e] = 0;
+        uint32_t k = 0;
+#pragma unroll
+        for (int u = 0; u < HELD; u += 4) k = u == i ? key[u + e] : k;
+        if (row_of(j0, i + e) < len) quad[e] = (k > prefix ? 1u : 0u) + (k == prefix ? 1u << 16 : 0u);
+        sum += quad[e];
+      }
+      const uint32_t s = wave_scan_u32(sum);
+      uint32_t at = before + s - sum;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t eq = n_equal + (at >> 16), place = n_above + (at & 0xffffu) + min(eq, want);
+        if (quad[e] == 1u || (quad[e] != 0 && eq < want)) out[place] = row_of(j0, i + e);
+        at += quad[e];
+      }
+      before += lane_63(s);
+    }
+    n_above += all & 0xffffu;
+    n_equal += all >> 16;
   }
 }
 
@@ -288,7 +340,7 @@ __global__ __launch_bounds__(IN_PLACE ? 1024 : 256) void gather_kernel(Cache fro
       }
       top = fmaxf(top, m * s[i]);
     }
-    const int e = kv8_exponent(wave_max(top));
+    const int e = kv8_exponent(wave_most_f32(top));
     const float inv = kv8_pow2(-e);
     if constexpr (IN_PLACE) __syncthreads();  // (every load of these blocks has arrived: their values are in use above)
     bool any = false;
@@ -373,8 +425,12 @@ extern "C" md_status md_kv8_evict(const md_kv8_cache* from, const md_kv8_cache* 
     MD_CHECK_ARG(caches_apart(from, to) && (!a->weights_out || apart(a->weights, wn, a->weights_out, wm)));
   }
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(select_kernel, dim3(from->kv_heads, a->batch), dim3(SEL), 0, s, a->weights, a->slot, a->kv_len, a->kept, from->slots, from->ctx,
-                     from->kv_heads, a->keep, a->first, a->recent);
+#define MD_SELECT(HELD, COPIES)                                                                                                                    \
+  hipLaunchKernelGGL((select_kernel<HELD, COPIES>), dim3(from->kv_heads, a->batch), dim3(SEL), 0, s, a->weights, a->slot, a->kv_len, a->kept,      \
+                     from->slots, from->ctx, from->kv_heads, a->keep, a->first, a->recent)
+  if (from->ctx <= 4 * SEL) MD_SELECT(4, 2);
+  else MD_SELECT(32, 8);
+#undef MD_SELECT
   const int n_blocks = (a->keep + BLK - 1) / BLK;
   const int64_t heads2 = (int64_t)a->batch * from->kv_heads * 2, tasks = in_place ? heads2 : heads2 * n_blocks, groups = in_place ? tasks : (tasks + 3) / 4;
   MD_CHECK_ARG(groups <= 0x7fffffff);

@@ -45,6 +45,8 @@ struct Params {
   uint32_t per_group, all;  // 2^32 / group rounded up and 0; 0 and ~0 for a group of 1
   uint32_t q_sign;          // xor of two bf16 queries: a negative scale is taken as its magnitude and the queries negated, so that scores rise with products
   float scale_log2, decay;
+  float *scores;            // of few columns, with weights: [batch][kv_heads][cols][max_len to a whole block], in units of log2
+  int score_rows, join_groups;
   float *part, *part_ml, *lse, *weights;  // part: [batch][kv_heads][cols][splits][head_dim], part_ml: ... [splits][2], lse: [batch][kv_heads][cols]
 };
 
@@ -251,32 +253,25 @@ __device__ __forceinline__ void store_column(const Params& p, int b, int kvh, in
   if (p.lse && first) p.lse[c] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
-// The columns of a wave: queries, how many keys each sees, and the most and the least of them
+// The columns of a wave: queries, how many keys each sees, and the most and the least of them (a later query never sees less)
 template <int HD, int NT>
 __device__ __forceinline__ void load_columns(const Params& p, const Seq& sq, int b, int kvh, int col0, int n_cols, int lane, bf16x8 (&qf)[NT][HD / 32], int (&lim)[NT],
                                              int& most, int& least) {
-  most = 0;
-  least = 0x7fffffff;
+  least = limit_of(p, sq, sq.pos0 + query_of(p, col0));
+  most = col0 < n_cols ? limit_of(p, sq, sq.pos0 + query_of(p, min(col0 + 16 * NT, n_cols) - 1)) : 0;
+  most = __builtin_amdgcn_readfirstlane(most);
+  least = __builtin_amdgcn_readfirstlane(least);
 #pragma unroll
   for (int ct = 0; ct < NT; ++ct) {
     const int col = col0 + ct * 16 + (lane & 15);
     load_query<HD>(p, b, kvh, col, sq.rows, lane >> 4, qf[ct]);
     lim[ct] = col < n_cols ? limit_of(p, sq, sq.pos0 + query_of(p, col)) : 0;
-    most = max(most, lim[ct]);
-    if (col < n_cols) least = min(least, lim[ct]);
   }
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    most = max(most, __shfl_xor(most, o, 64));
-    least = min(least, __shfl_xor(least, o, 64));
-  }
-  most = __builtin_amdgcn_readfirstlane(most);
-  least = __builtin_amdgcn_readfirstlane(least);
 }
 
-// Few columns: the four waves share NT column tiles and take every fourth block, registers only.
-template <int HD, int NT>
-__global__ __launch_bounds__(256) void decode_kernel(Params p) {
+// Few columns: the W waves share NT column tiles and take every W-th block, registers only.
+template <int HD, int NT, int W>
+__global__ __launch_bounds__(64 * W) void decode_kernel(Params p) {
   constexpr int VT = HD / 16;  // tiles of 16 coordinates of the output
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   const int split = blockIdx.x % p.splits, cg = blockIdx.x / p.splits, kvh = blockIdx.y, b = blockIdx.z;
@@ -321,7 +316,19 @@ __global__ __launch_bounds__(256) void decode_kernel(Params p) {
     f32x4 s[NT][2];
     scores<HD, 2, NT>(a, qf, s);
     f16x8 pf[NT];
-    softmax_block<NT, VT>(s, pf, acc, m, l, lim, key0 + BLK > least, key0, q, p.scale_log2 * kv8_pow2(f.ke - 127), (float)(f.ve - 127), kv8_pow2(127 - f.ve));
+    const float ck = p.scale_log2 * kv8_pow2(f.ke - 127);
+    if (p.scores) {
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct) {
+        const int col = col0 + ct * 16 + r;
+        float* out = p.scores + (((int64_t)b * p.kv_heads + kvh) * p.cols + col) * p.score_rows + key0 + 4 * q;
+        if (col < n_cols) {
+          *(f32x4*)out = s[ct][0] * ck;
+          *(f32x4*)(out + 16) = s[ct][1] * ck;
+        }
+      }
+    }
+    softmax_block<NT, VT>(s, pf, acc, m, l, lim, key0 + BLK > least, key0, q, ck, (float)(f.ve - 127), kv8_pow2(127 - f.ve));
 #pragma unroll
     for (int c = 0; c < HD / 64; ++c) {
       const uint32_t w0[4] = {f.v[0][c], f.v[1][c], f.v[2][c], f.v[3][c]}, w1[4] = {f.v[4][c], f.v[5][c], f.v[6][c], f.v[7][c]};
@@ -342,19 +349,19 @@ __global__ __launch_bounds__(256) void decode_kernel(Params p) {
   if (first < end) {
     Block<HD> f0, f1;
     load_block<HD>(f0, k, v, ke, ve, first, lane);
-    for (int block = first; block < end; block += 8) {
-      load_block<HD>(f1, k, v, ke, ve, min(block + 4, end - 1), lane);
+    for (int block = first; block < end; block += 2 * W) {
+      load_block<HD>(f1, k, v, ke, ve, min(block + W, end - 1), lane);
       step(f0, block);
-      load_block<HD>(f0, k, v, ke, ve, min(block + 8, end - 1), lane);
-      if (block + 4 < end) step(f1, block + 4);
+      load_block<HD>(f0, k, v, ke, ve, min(block + 2 * W, end - 1), lane);
+      if (block + W < end) step(f1, block + W);
     }
   }
 #pragma unroll
   for (int ct = 0; ct < NT; ++ct) l[ct] = over_q_sum(l[ct]);
 
   // a lane holds, of column r, coordinates VT (4 q + i) + t at acc[t][i]
-  __shared__ float so[4][VT * 4][64];
-  __shared__ float sm[4][16], sl[4][16];
+  __shared__ float so[W][VT * 4][64];
+  __shared__ float sm[W][16], sl[W][16];
   for (int ct = 0; ct < NT; ++ct) {
     if (ct) __syncthreads();
 #pragma unroll
@@ -366,22 +373,23 @@ __global__ __launch_bounds__(256) void decode_kernel(Params p) {
       sl[wave][r] = l[ct];
     }
     __syncthreads();
-    float f[4], mm = NO_MAX, ll = 0.f;
+    if (wave >= 4) continue;
+    float f[W], mm = NO_MAX, ll = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm[w][r]);
+    for (int w = 0; w < W; ++w) mm = fmaxf(mm, sm[w][r]);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < W; ++w) {
       f[w] = __builtin_amdgcn_exp2f(sm[w][r] - mm);
       ll = __builtin_fmaf(sl[w][r], f[w], ll);
     }
     const int col = col0 + ct * 16 + r;
-    if (col < n_cols) {  // wave i: coordinates VT (4 q + i) ..
+    if (col < n_cols) {  // wave i < 4: coordinates VT (4 q + i) ..
       float out[VT];
 #pragma unroll
       for (int t = 0; t < VT; ++t) {
         out[t] = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) out[t] = __builtin_fmaf(so[w][t * 4 + wave][lane], f[w], out[t]);
+        for (int w = 0; w < W; ++w) out[t] = __builtin_fmaf(so[w][t * 4 + wave][lane], f[w], out[t]);
       }
       store_column<HD, VT>(p, b, kvh, col, split, VT * (4 * q + wave), out, mm, ll, q == 0 && wave == 0);
     }
@@ -550,33 +558,93 @@ __global__ __launch_bounds__(256, 3) void prompt_kernel(Params p) {
   }
 }
 
-// Joins the workgroups that shared a column's keys: one wave per column, in the splits' order.
+// What the workgroups that shared a column's keys have: lane s holds split s's maximum as a factor; the common maximum, the sum
+__device__ __forceinline__ float join_factor(const float* __restrict__ ml, int splits, int lane, float& m, float& l) {
+  const float ms = lane < splits ? ml[2 * lane] : NO_MAX, ls = lane < splits ? ml[2 * lane + 1] : 0.f;
+  m = wave_max(ms);
+  const float f = __builtin_amdgcn_exp2f(ms - m);
+  l = wave_sum(ls * f);
+  return f;
+}
+
+// After workgroups that shared keys.  The first join_groups workgroups of a head: one wave per column, its parts added in the splits' order.  The others (few
+// columns with weights): every row's softmax weights from the scores that the attention kernel left, 1024 rows each.
 template <int HD>
 __global__ __launch_bounds__(256) void join_kernel(Params p) {
   constexpr int N = HD / 64;
-  const int lane = threadIdx.x & 63, col = blockIdx.x * 4 + (threadIdx.x >> 6), kvh = blockIdx.y, b = blockIdx.z;
-  const int rows = p.q_rows ? min(max(p.q_rows[b], 0), p.q_len) : p.q_len;
-  if (col >= rows * p.group) return;
-  const int64_t c0 = ((int64_t)b * p.kv_heads + kvh) * p.cols + col;
-  const float* ml = p.part_ml + c0 * p.splits * 2;
-  const float* part = p.part + c0 * p.splits * HD + lane * N;
-  float m = NO_MAX, l = 0.f, o[N] = {};
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[2 * s]);
-  for (int s = 0; s < p.splits; ++s) {
-    const float f = __builtin_amdgcn_exp2f(ml[2 * s] - m);
-    l = __builtin_fmaf(ml[2 * s + 1], f, l);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, kvh = blockIdx.y, b = blockIdx.z;
+  const int64_t bh = (int64_t)b * p.kv_heads + kvh;
+  const Seq sq = sequence(p, b);
+  const int n_cols = sq.rows * p.group;
+  if ((int)blockIdx.x < p.join_groups) {
+    const int col = blockIdx.x * 4 + wave;
+    if (col >= n_cols) return;
+    const int64_t c0 = bh * p.cols + col;
+    float m, l, o[N] = {};
+    const float f = join_factor(p.part_ml + c0 * p.splits * 2, p.splits, lane, m, l);
+    const float* part = p.part + c0 * p.splits * HD + lane * N;
+    for (int s = 0; s < p.splits; s += 8) {
+      float x[8][N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = __builtin_fmaf(part[(int64_t)s * HD + i], f, o[i]);
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[u][i] = part[(int64_t)min(s + u, p.splits - 1) * HD + i];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float fu = s + u < p.splits ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s + u)) : 0.f;
+        if (s + u < p.splits) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) o[i] = __builtin_fmaf(x[u][i], fu, o[i]);
+        }
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int t = query_of(p, col), g = col - t * p.group;
+    bf16_t* out = p.o + (int64_t)b * p.o_bs + (int64_t)t * p.o_ts + (int64_t)(kvh * p.group + g) * p.o_hs + lane * N;
+    if constexpr (N == 1) *out = f2bf(o[0] * inv);
+    else *(uint32_t*)out = pack_bf16x2(o[0] * inv, o[1] * inv);
+    if (p.lse && lane == 0) p.lse[c0] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    return;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int t = query_of(p, col), g = col - t * p.group;
-  bf16_t* out = p.o + (int64_t)b * p.o_bs + (int64_t)t * p.o_ts + (int64_t)(kvh * p.group + g) * p.o_hs + lane * N;
+  __shared__ float lse[32];
+  __shared__ int lims[32];
+  const int first = (blockIdx.x - p.join_groups) * 1024;
+  if (first >= sq.len) return;
+  for (int col = wave; col < n_cols; col += 4) {
+    const int64_t c0 = bh * p.cols + col;
+    float x;
+    if (p.splits > 1) {
+      float m, l;
+      join_factor(p.part_ml + c0 * p.splits * 2, p.splits, lane, m, l);
+      x = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    } else {
+      x = p.lse[c0];
+    }
+    if (lane == 0) {
+      lse[col] = x;
+      lims[col] = limit_of(p, sq, sq.pos0 + query_of(p, col));
+    }
+  }
+  __syncthreads();
+  const int key = first + (int)threadIdx.x * 4;
+  if (key >= sq.len) return;
+  const float* sc = p.scores + bh * p.cols * p.score_rows + key;
+  float w[4] = {};
+  for (int col = 0; col < n_cols; ++col) {
+    const float ls = lse[col];
+    const int lim = lims[col];
+    if (key >= lim) continue;  // (its scores may not be there)
+    const f32x4 s = *(const f32x4*)(sc + (int64_t)col * p.score_rows);
 #pragma unroll
-  for (int i = 0; i < N; ++i) out[i] = f2bf(o[i] * inv);
-  if (p.lse && lane == 0) p.lse[c0] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    for (int i = 0; i < 4; ++i) w[i] += key + i < lim ? __builtin_amdgcn_exp2f(s[i] - ls) : 0.f;
+  }
+  float* out = p.weights + ((int64_t)sq.slot * p.kv_heads + kvh) * p.ctx + key;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (key + i < sq.len) out[i] = p.decay == 0.f ? w[i] : __builtin_fmaf(p.decay, out[i], w[i]);
 }
 
-// The weight that every row got.  A wave holds 64 keys as operands; the columns that see them pass by, 64 at a time through LDS.  Of a workgroup's four
+// The weight that every row got from many columns.  A wave holds 64 keys as operands; the columns that see them pass by, 64 at a time through LDS.  Of a workgroup's four
 // waves two have the same keys, one for each half of the columns (workgroups of 128 keys: more of them, for the sake of balance).  The
 // scores are the attention kernel's again (the same products in the same order), exp2(score - lse) is their softmax.
 template <int HD>
@@ -690,12 +758,15 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(Params p) {
 
 constexpr int PROMPT_NT = 2;
 
-// How a call is cut.  Up to 32 columns a wave's tiles would stand empty, and its keys are what there is to read: the four waves of a
-// workgroup share them.  Splits: enough workgroups for 256 CUs of 4 workgroups each, none with less than 8 blocks (decode) or 16.
+// How a call is cut.  Up to 32 columns a wave's tiles would stand empty, and its keys are what there is to read: the waves of a workgroup share
+// them.  Splits: enough workgroups for 256 CUs of 4 workgroups each, none with less than 8 blocks (decode) or 16.  Where that would be a second launch
+// for little work, workgroups of 16 waves (8 where registers allow no more) take all keys of a head: one per CU at most, up to two blocks a wave,
+// eight where half of the CUs have one (us, one launch against two: 1 x 32 heads of 64, 800 keys 7.0 / 8.2, 2000 keys 9.5 / 8.3; 8 x 32 heads 7.9 / 10.3
+// and 13.3 / 17.1, 12 x 32 heads 14.0 / 13.7).
 struct Plan {
   bool decode;
-  int nt, col_groups, splits, cols;
-  size_t part, ml, lse, bytes;
+  int nt, waves, col_groups, splits, cols, score_rows;
+  size_t part, ml, lse, scores, bytes;
 };
 
 Plan plan_of(const md_kv8_cache* c, const md_kv8_attn_args* a) {
@@ -707,13 +778,17 @@ Plan plan_of(const md_kv8_cache* c, const md_kv8_attn_args* a) {
   pl.col_groups = (pl.cols + per - 1) / per;
   const int max_len = a->max_len > 0 ? std::min(a->max_len, c->ctx) : c->ctx, blocks = (max_len + BLK - 1) / BLK;
   const int64_t groups = (int64_t)pl.col_groups * c->kv_heads * a->batch;
+  const int wide = pl.nt == 1 && c->head_dim == 64 ? 16 : 8;
+  pl.waves = pl.decode && groups <= 256 && blocks >= 16 && blocks <= (groups >= 128 ? 8 : 2) * wide ? wide : 4;
   const int64_t want = ((pl.decode ? 1024 : 512) + groups - 1) / groups, most = std::max(1, blocks / (pl.decode ? 8 : 16));
-  pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 64}));
+  pl.splits = pl.waves > 4 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 64}));
   const int64_t cols = (int64_t)a->batch * c->kv_heads * pl.cols;
   pl.part = 0;
   pl.ml = pl.splits > 1 ? cols * pl.splits * c->head_dim * 4 : 0;
   pl.lse = pl.ml + (pl.splits > 1 ? cols * pl.splits * 2 * 4 : 0);
-  pl.bytes = pl.lse + (a->weights ? cols * 4 : 0);
+  pl.scores = (pl.lse + (a->weights ? cols * 4 : 0) + 15) & ~(size_t)15;
+  pl.score_rows = blocks * BLK;
+  pl.bytes = pl.scores + (a->weights && pl.decode ? (size_t)cols * pl.score_rows * 4 : 0);
   return pl;
 }
 
@@ -767,31 +842,47 @@ extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_at
   p.part_ml = (float*)(ws + pl.ml);
   p.lse = a->weights ? (float*)(ws + pl.lse) : nullptr;
   p.weights = a->weights;
+  p.scores = a->weights && pl.decode ? (float*)(ws + pl.scores) : nullptr;
+  p.score_rows = pl.score_rows;
+  p.join_groups = pl.splits > 1 ? (pl.cols + 3) / 4 : 0;
   const int64_t groups = (int64_t)pl.col_groups * pl.splits, all = groups * cache->kv_heads * a->batch;
   MD_CHECK_ARG(all <= 0x7fffffff);
   const dim3 grid(groups, cache->kv_heads, a->batch), block(256);
   hipStream_t s = (hipStream_t)stream;
   if (pl.decode) {
+#define MD_DECODE(HD, NT, W) hipLaunchKernelGGL((decode_kernel<HD, NT, W>), grid, dim3(64 * W), 0, s, p)
     if (cache->head_dim == 64) {
-      if (pl.nt == 1) hipLaunchKernelGGL((decode_kernel<64, 1>), grid, block, 0, s, p);
-      else hipLaunchKernelGGL((decode_kernel<64, 2>), grid, block, 0, s, p);
+      if (pl.nt == 1) {
+        if (pl.waves > 4) MD_DECODE(64, 1, 16);
+        else MD_DECODE(64, 1, 4);
+      } else {
+        if (pl.waves > 4) MD_DECODE(64, 2, 8);
+        else MD_DECODE(64, 2, 4);
+      }
     } else {
-      if (pl.nt == 1) hipLaunchKernelGGL((decode_kernel<128, 1>), grid, block, 0, s, p);
-      else hipLaunchKernelGGL((decode_kernel<128, 2>), grid, block, 0, s, p);
+      if (pl.nt == 1) {
+        if (pl.waves > 4) MD_DECODE(128, 1, 8);
+        else MD_DECODE(128, 1, 4);
+      } else {
+        if (pl.waves > 4) MD_DECODE(128, 2, 8);
+        else MD_DECODE(128, 2, 4);
+      }
     }
+#undef MD_DECODE
   } else if (cache->head_dim == 64) {
     hipLaunchKernelGGL((prompt_kernel<64, PROMPT_NT>), dim3(all), block, 0, s, p);
   } else {
     hipLaunchKernelGGL((prompt_kernel<128, PROMPT_NT>), dim3(all), block, 0, s, p);
   }
   MD_TRY(md_launch_status());
-  if (pl.splits > 1) {
-    const dim3 jg((pl.cols + 3) / 4, cache->kv_heads, a->batch);
+  const int tail = p.join_groups + (p.scores ? (p.max_len + 1023) / 1024 : 0);
+  if (tail) {
+    const dim3 jg(tail, cache->kv_heads, a->batch);
     if (cache->head_dim == 64) hipLaunchKernelGGL(join_kernel<64>, jg, block, 0, s, p);
     else hipLaunchKernelGGL(join_kernel<128>, jg, block, 0, s, p);
     MD_TRY(md_launch_status());
   }
-  if (a->weights) {
+  if (a->weights && !pl.decode) {
     const dim3 wg((p.max_len + 127) / 128, cache->kv_heads, a->batch);
     if (cache->head_dim == 64) hipLaunchKernelGGL(weights_kernel<64>, wg, block, 0, s, p);
     else hipLaunchKernelGGL(weights_kernel<128>, wg, block, 0, s, p);

@@ -14,7 +14,7 @@ from typing import NamedTuple, Optional, Sequence
 import torch
 
 from . import _lib
-from .block_cache import _need, _on, _stream
+from .block_cache import _launch, _need
 
 MAX_BEAMS = _lib.MD_MAX_BEAMS
 _DTYPES = {torch.bfloat16: _lib.MD_DTYPE_BF16, torch.float32: _lib.MD_DTYPE_F32}
@@ -51,18 +51,17 @@ def select_beams(logits: torch.Tensor, scores: torch.Tensor, ended: Optional[tor
     if logits.stride(1) != 1 or logits.stride(0) < vocab:
         raise ValueError(f"logits of strides {logits.stride()}: rows have to be contiguous and apart")
     dev, shape = _gpu(logits, "select_beams"), (batch, beams)
-    addresses = [None if t is None else _need(t, name, dtype, dev, shape)
-                 for t, name, dtype in ((scores, "scores", torch.float32), (ended, "ended", torch.int32), (rank_weight, "rank_weight", torch.float32))]
-    ints = torch.empty(3, batch, beams, dtype=torch.int32, device=dev)
+    tokens, parents, stop = torch.empty((3, batch, beams), dtype=torch.int32, device=dev).unbind(0)
     new = torch.empty(shape, dtype=torch.float32, device=dev)
-    tokens, parents, stop = ints.unbind(0)
     lib = _lib.load()
-    with _on(dev):
-        need = lib.md_beam_workspace_bytes(batch, beams, vocab)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        a = _lib.MdBeamArgs(logits.data_ptr(), logits.stride(0), _DTYPES[logits.dtype], batch, beams, vocab, suppress_id, max(end_id, -1), *addresses,
-                            tokens.data_ptr(), parents.data_ptr(), new.data_ptr(), stop.data_ptr(), ws.data_ptr(), need)
-        _lib.check(lib.md_beam_select(C.byref(a), _stream(dev)), "md_beam_select")
+    need = lib.md_beam_workspace_bytes(batch, beams, vocab)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    at = tokens.data_ptr()
+    a = _lib.MdBeamArgs(logits.data_ptr(), logits.stride(0), _DTYPES[logits.dtype], batch, beams, vocab, suppress_id, max(end_id, -1),
+                        _need(scores, "scores", torch.float32, dev, shape), None if ended is None else _need(ended, "ended", torch.int32, dev, shape),
+                        None if rank_weight is None else _need(rank_weight, "rank_weight", torch.float32, dev, shape),
+                        at, at + 4 * batch * beams, new.data_ptr(), at + 8 * batch * beams, ws.data_ptr(), need)
+    _launch(dev.index, "md_beam_select", lib.md_beam_select, C.byref(a))
     return BeamChoice(tokens, parents, new, stop)
 
 
@@ -107,14 +106,12 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, into: 
             continue
         at = slot_dim % src.dim()
         a = _runs(src, at, name)
-        b = a if src is dst else _runs(dst, at, name)
+        b = a if src.stride() == dst.stride() else _runs(dst, at, name)
         if (a[1][0], a[2][0], a[3]) != (b[1][0], b[2][0], b[3]):
             raise ValueError(f"{name}: strides {src.stride()} into {dst.stride()}")
         parts.append((src.data_ptr(), dst.data_ptr(), a[0], b[0], a[1][1], b[1][1], a[2][1], b[2][1], a[3], a[1][0], a[2][0]))
     if not parts:
         return
     dev = _gpu(parents, "reorder_states")
-    lib = _lib.load()
-    with _on(dev):
-        _lib.check(lib.md_state_reorder((_lib.MdStatePart * len(parts))(*parts), len(parts), _need(parents, "parents", torch.int32, dev), batch, beams,
-                                        _stream(dev)), "md_state_reorder")
+    _launch(dev.index, "md_state_reorder", _lib.load().md_state_reorder, (_lib.MdStatePart * len(parts))(*parts), len(parts),
+            _need(parents, "parents", torch.int32, dev, (batch, beams)), batch, beams)

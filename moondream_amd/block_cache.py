@@ -13,7 +13,6 @@ Like torch's operators on tensors of another stream, a call does not wait for wo
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import math
 from typing import Optional, Tuple
@@ -26,19 +25,24 @@ BLOCK = _lib.MD_KV8_BLOCK
 _BF16, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
 
 
-def _on(device: torch.device):
-    """The launches' device: tensors of another device than the current one are served on theirs."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+_current_device, _raw_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _launch(index: int, what: str, call, *args) -> None:
+    """An entry point on the current stream of device ``index``, which is made the current one if it is not."""
+    if _current_device() == index:
+        status = call(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = call(*args, _raw_stream(index))
+    if status:
+        _lib.check(status, what)
 
 
-def _need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, shape: Optional[tuple] = None) -> int:
+def _need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, shape: tuple) -> int:
     """The address of a contiguous tensor that is what it has to be."""
-    if t.dtype != dtype or t.device != device or (shape is not None and t.shape != shape) or not t.is_contiguous():
-        raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device}, wanted contiguous {shape if shape is not None else ''} {dtype} on {device}")
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device}, wanted contiguous {shape} {dtype} on {device}")
     return t.data_ptr()
 
 
@@ -80,7 +84,9 @@ class BlockCache:
         self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
         self.slots, self.kv_heads, self.ctx, self.head_dim = slots, heads, ctx, dim
         self.device = torch.device("cuda", k.device.index if k.device.index is not None else torch.cuda.current_device())
+        self._index = self.device.index
         self._lib = _lib.load()
+        self._workspaces: dict = {}  # bytes that calls of a shape need
         stride = (k.stride(0), k_exp.stride(0)) if slots > 1 else (heads * ctx * dim, heads * ctx // BLOCK)
         self._struct = _lib.MdKv8Cache(k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), stride[0], stride[1], slots, ctx, heads, dim)
         self._ref = C.byref(self._struct)
@@ -92,30 +98,29 @@ class BlockCache:
         if batch <= 0 or (slot is None and batch > self.slots):
             raise ValueError(f"a batch of {batch} sequences in {self.slots} slots")
 
-    def _rows_of(self, t: torch.Tensor, name: str, heads: Optional[int]) -> torch.Tensor:
+    def _rows_of(self, t: torch.Tensor, name: str, heads: Optional[int]) -> tuple:
+        """The strides of bf16 rows that are as the kernels take them."""
         if t.dim() != 4 or t.dtype != _BF16 or t.device != self.device or t.shape[3] != self.head_dim or (heads is not None and t.shape[2] != heads):
             raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device}, wanted [batch, tokens, {heads or 'heads'}, {self.head_dim}] bfloat16 on {self.device}")
         s = t.stride()
         if t.data_ptr() % 16 or (s[0] | s[1] | s[2]) % 8 or s[3] != 1:
             raise ValueError(f"{name}: rows of head_dim have to be contiguous and 16-byte aligned (strides {s})")
-        return t
+        return s
 
     def append(self, k: torch.Tensor, v: torch.Tensor, row0: torch.Tensor, new: Optional[torch.Tensor] = None, slot: Optional[torch.Tensor] = None) -> None:
         """Rows row0[b] .. of every sequence from bf16 ``k``, ``v`` [batch, tokens, kv_heads, head_dim] (views of a projection's rows will do; keys
         rotated already); ``new``: how many of the tokens count, per sequence.  Rows past ``ctx`` are dropped.  A slot at most once."""
-        self._rows_of(k, "k", self.kv_heads)
-        self._rows_of(v, "v", self.kv_heads)
+        ks, vs = self._rows_of(k, "k", self.kv_heads), self._rows_of(v, "v", self.kv_heads)
         batch, tokens = k.shape[:2]
         if v.shape != k.shape:
             raise ValueError(f"keys {tuple(k.shape)} and values {tuple(v.shape)}")
         self._batch(batch, slot)
         if tokens == 0:
             return
-        ks, vs = k.stride(), v.stride()
-        with _on(self.device):
-            _lib.check(self._lib.md_kv8_append(self._ref, k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
-                                               self._per_sequence(slot, "slot", batch), self._per_sequence(row0, "row0", batch),
-                                               self._per_sequence(new, "new", batch), batch, tokens, _stream(self.device)), "md_kv8_append")
+        of = (batch,)
+        _launch(self._index, "md_kv8_append", self._lib.md_kv8_append, self._ref, k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
+                None if slot is None else _need(slot, "slot", _I32, self.device, of), _need(row0, "row0", _I32, self.device, of),
+                None if new is None else _need(new, "new", _I32, self.device, of), batch, tokens)
 
     def read(self, row0: Optional[torch.Tensor], rows: int, kv_len: Optional[torch.Tensor] = None, slot: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """Rows row0[b] .. row0[b] + rows - 1 (None: from 0) as bf16 [batch, kv_heads, rows, head_dim] keys and values, exactly what the codes stand
@@ -125,12 +130,10 @@ class BlockCache:
         self._batch(batch, slot)
         if rows < 0:
             raise ValueError(f"{rows} rows")
-        k, v = (torch.empty(batch, self.kv_heads, rows, self.head_dim, dtype=_BF16, device=self.device) for _ in range(2))
+        k, v = torch.empty((2, batch, self.kv_heads, rows, self.head_dim), dtype=_BF16, device=self.device).unbind(0)
         if rows:
-            with _on(self.device):
-                _lib.check(self._lib.md_kv8_read(self._ref, self._per_sequence(slot, "slot", batch), self._per_sequence(row0, "row0", batch),
-                                                 self._per_sequence(kv_len, "kv_len", batch), batch, rows, k.data_ptr(), v.data_ptr(),
-                                                 _stream(self.device)), "md_kv8_read")
+            _launch(self._index, "md_kv8_read", self._lib.md_kv8_read, self._ref, self._per_sequence(slot, "slot", batch), self._per_sequence(row0, "row0", batch),
+                    self._per_sequence(kv_len, "kv_len", batch), batch, rows, k.data_ptr(), v.data_ptr())
         return k, v
 
     def _weights(self, w: Optional[torch.Tensor], name: str) -> Optional[int]:
@@ -145,7 +148,7 @@ class BlockCache:
         ``prefix_len`` rows all of these.  ``q_rows``: how many of the queries count (the others' outputs stay as ``out`` has them; without
         ``out`` they are zeros).  ``max_len``: no sequence is longer (sizes the launch; longer ones are cut).  ``scale``: 1 / sqrt(head_dim).
         ``weights`` (fp32 [slots, kv_heads, ctx]) <- decay * weights + the softmax weight that every row got in this call."""
-        self._rows_of(q, "q", None)
+        qs = self._rows_of(q, "q", None)
         batch, tokens, heads, dim = q.shape
         if heads == 0 or heads % self.kv_heads:
             raise ValueError(f"{heads} query heads over {self.kv_heads} key heads")
@@ -154,24 +157,26 @@ class BlockCache:
             raise ValueError(f"max_len {max_len}, prefix_len {prefix_len}")
         if out is None:
             out = (torch.empty if q_rows is None else torch.zeros)(q.shape, dtype=_BF16, device=self.device)
-        elif out.shape != q.shape:
-            raise ValueError(f"out: {tuple(out.shape)}, wanted {tuple(q.shape)}")
-        self._rows_of(out, "out", heads)
+            os = out.stride()
+        else:
+            if out.shape != q.shape:
+                raise ValueError(f"out: {tuple(out.shape)}, wanted {tuple(q.shape)}")
+            os = self._rows_of(out, "out", heads)
         if tokens == 0:
             return out
-        qs, os = q.stride(), out.stride()
+        longest = 0 if max_len is None else min(max_len, self.ctx)
         a = _lib.MdKv8AttnArgs(q.data_ptr(), qs[0], qs[1], qs[2], out.data_ptr(), os[0], os[1], os[2], batch, heads, tokens,
                                self._per_sequence(slot, "slot", batch), self._per_sequence(q_pos0, "q_pos0", batch),
-                               self._per_sequence(q_rows, "q_rows", batch), self._per_sequence(kv_len, "kv_len", batch),
-                               0 if max_len is None else min(max_len, self.ctx), min(prefix_len, self.ctx), 1.0 / math.sqrt(dim) if scale is None else scale,
-                               decay, self._weights(weights, "weights"), None, 0)
-        ref = C.byref(a)
-        with _on(self.device):
-            need = self._lib.md_kv8_attention_workspace_bytes(self._ref, ref)
-            if need:
-                ws = torch.empty(need, dtype=_U8, device=self.device)
-                a.workspace, a.workspace_bytes = ws.data_ptr(), need
-            _lib.check(self._lib.md_kv8_attention(self._ref, ref, _stream(self.device)), "md_kv8_attention")
+                               self._per_sequence(q_rows, "q_rows", batch), _need(kv_len, "kv_len", _I32, self.device, (batch,)), longest,
+                               min(prefix_len, self.ctx), 1.0 / math.sqrt(dim) if scale is None else scale, decay, self._weights(weights, "weights"), None, 0)
+        shape = (batch, heads, tokens, longest, weights is None)
+        need = self._workspaces.get(shape)
+        if need is None:
+            need = self._workspaces[shape] = self._lib.md_kv8_attention_workspace_bytes(self._ref, C.byref(a))
+        if need:
+            ws = torch.empty(need, dtype=_U8, device=self.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        _launch(self._index, "md_kv8_attention", self._lib.md_kv8_attention, self._ref, C.byref(a))
         return out
 
     def evict(self, weights: torch.Tensor, kv_len: torch.Tensor, keep: int, first: int = 0, recent: int = 0, slot: Optional[torch.Tensor] = None,
@@ -195,6 +200,5 @@ class BlockCache:
         length = torch.empty(batch, dtype=_I32, device=self.device)
         a = _lib.MdKv8EvictArgs(w, w if into is None else to._weights(into_weights, "into_weights"), self._per_sequence(slot, "slot", batch),
                                 self._per_sequence(kv_len, "kv_len", batch), length.data_ptr(), kept.data_ptr(), batch, keep, first, recent)
-        with _on(self.device):
-            _lib.check(self._lib.md_kv8_evict(self._ref, to._ref, C.byref(a), _stream(self.device)), "md_kv8_evict")
+        _launch(self._index, "md_kv8_evict", self._lib.md_kv8_evict, self._ref, to._ref, C.byref(a))
         return kept, length

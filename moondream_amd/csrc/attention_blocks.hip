@@ -17,6 +17,7 @@
 // Few columns (decode): the four waves of a workgroup share a column tile and take every fourth block, several workgroups share the keys, and
 // a second kernel joins their (O, m, l).  Many columns (prompts): every wave has its own columns, the converted operands come through LDS.
 #include "block_cache.hpp"
+#include "wave_ops.hpp"
 
 #include <algorithm>
 
@@ -46,7 +47,8 @@ struct Params {
   uint32_t q_sign;          // xor of two bf16 queries: a negative scale is taken as its magnitude and the queries negated, so that scores rise with products
   float scale_log2, decay;
   float *scores;            // of few columns, with weights: [batch][kv_heads][cols][max_len to a whole block], in units of log2
-  int score_rows, join_groups;
+  int score_rows, join_groups, batch, by_length, col_splits;
+  float* wpart;             // of many columns shared out: [col_splits][batch][kv_heads][max_len to a whole block]
   float *part, *part_ml, *lse, *weights;  // part: [batch][kv_heads][cols][splits][head_dim], part_ml: ... [splits][2], lse: [batch][kv_heads][cols]
 };
 
@@ -396,6 +398,37 @@ __global__ __launch_bounds__(64 * W) void decode_kernel(Params p) {
   }
 }
 
+// The workgroup of rank `rank` among all sequences' groups of PER columns, the ones that reach farthest into their cache first (a batch's sequences differ
+// in length, and what starts last should be short).  Group cg of a sequence reaches to row pos0 + (cg + 1) PER / group, in columns: base + (cg + 1) PER.
+// Lane i counts sequence i's groups from a bound on; the bound is found by halving.  False: there are not so many groups.
+template <int PER>
+__device__ __forceinline__ bool longest_first(const Params& p, int rank, int lane, int& b, int& cg) {
+  const Seq s = sequence(p, min(lane, p.batch - 1));
+  const int n = lane < p.batch ? (s.rows * p.group + PER - 1) / PER : 0, base = s.pos0 * p.group;
+  const auto sum = [](int v) { return (int)lane_63(wave_scan_u32((uint32_t)v)); };
+  const auto from = [&](int bound) { return max(0, n - max(0, (bound - base + PER - 1) / PER - 1)); };
+  if (rank >= sum(n)) return false;
+  int hi = n ? base + n * PER : -0x40000000, lo = n ? base + PER : 0x40000000;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    hi = max(hi, __shfl_xor(hi, o, 64));
+    lo = min(lo, __shfl_xor(lo, o, 64));
+  }
+  while (lo < hi) {
+    const int mid = lo + (hi - lo + 1) / 2;
+    if (sum(mid > base ? from(mid) : n) > rank) lo = mid;
+    else hi = mid - 1;
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  const int off = lo - base;
+  const bool here = n && off > 0 && off % PER == 0 && off / PER <= n;
+  uint64_t who = __ballot(here);
+  for (int skip = rank - sum(lo + 1 > base ? from(lo + 1) : n); skip > 0; --skip) who &= who - 1;
+  b = __builtin_ctzll(who);
+  cg = __builtin_amdgcn_readlane(off, b) / PER - 1;
+  return true;
+}
+
 // Many columns: every wave has its own NT tiles, and the four waves share the conversion: of the next two blocks, waves 0 and 1 bring the keys, 2 and 3
 // the values into LDS as the products' operands (16 bytes per lane, one operand after another: no bank conflicts either way), while all work on
 // the two before.  32 columns per wave: 48 and 64 need the registers of a third wave per SIMD, and larger workgroups even out worse over the CUs
@@ -403,24 +436,29 @@ __global__ __launch_bounds__(64 * W) void decode_kernel(Params p) {
 template <int HD, int NT>
 __global__ __launch_bounds__(256, 3) void prompt_kernel(Params p) {
   constexpr int VT = HD / 16, KF = 2 * (HD / 32), W = HD / 64;
-  __shared__ u32x4 frag[2][2][KF + VT][64];  // [turn][block][operand][lane]
-  __shared__ float scale[2][2][2];           // [turn][block]: a key's exponent as a factor, a value's as a number
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-  // Workgroup i runs on XCD i % 8.  Heads go to the XCDs in turn (a sequence's heads to all of them: sequences differ in length), and on an XCD the last
-  // queries, which see most, go first for all its heads.
-  const int per_head = p.splits * p.col_groups, heads = gridDim.x / per_head, full = heads / 8 * 8;
-  int id = blockIdx.x, head_id;
-  if (id < full * per_head) {
-    const int x = id & 7, n = full / 8;
-    id >>= 3;
-    head_id = id % n * 8 + x;
-    id /= n;
+  constexpr int SB = HD == 64 ? 2 : 1;        // blocks of a step: of one block a wave brings a tile of the keys, or 64 coordinates of the values
+  constexpr int T = SB, C = SB == 2 ? W : 1;  // tiles of keys and chunks of 64 coordinates of values that a wave brings
+  __shared__ u32x4 frag[2][SB][KF + VT][64];  // [turn][block][operand][lane]
+  __shared__ float scale[2][SB][2];           // [turn][block]: a key's exponent as a factor, a value's as a number
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
+  // Workgroup i runs on XCD i % 8, a head's workgroups on one XCD or few; of the columns that see most go first.
+  int id = blockIdx.x, kvh, b, cg;
+  const int split = id % p.splits;
+  id /= p.splits;
+  if (p.kv_heads % 8 == 0) {
+    const int n = p.kv_heads / 8;
+    kvh = (id >> 3) % n * 8 + (id & 7);
+    id = (id >> 3) / n;
   } else {
-    id -= full * per_head;
-    head_id = full + id % (heads - full);
-    id /= heads - full;
+    kvh = id % p.kv_heads;
+    id /= p.kv_heads;
   }
-  const int split = id % p.splits, cg = p.col_groups - 1 - id / p.splits, kvh = head_id % p.kv_heads, b = head_id / p.kv_heads;
+  if (p.by_length) {
+    if (!longest_first<64 * NT>(p, id, lane, b, cg)) return;
+  } else {
+    b = id % p.batch;
+    cg = p.col_groups - 1 - id / p.batch;
+  }
   const Seq sq = sequence(p, b);
   const int n_cols = sq.rows * p.group, wg0 = cg * 64 * NT, col0 = wg0 + wave * 16 * NT;
   if (wg0 >= n_cols) return;
@@ -445,83 +483,68 @@ __global__ __launch_bounds__(256, 3) void prompt_kernel(Params p) {
   const int64_t head = (int64_t)max(sq.slot, 0) * p.slot_stride + (int64_t)kvh * p.ctx * HD;
   const int64_t ehead = (int64_t)max(sq.slot, 0) * p.exp_stride + (int64_t)kvh * (p.ctx / BLK);
   const bool values = wave >= 2;
-  const int mine = wave & 1;  // of the two blocks
+  const int mine = wave & 1, part = SB == 2 ? 0 : mine, of = SB == 2 ? mine : 0;  // which tile or chunk, of which block
   const uint8_t* codes = (values ? p.v : p.k) + head;
   const uint8_t* exps = (values ? p.ve : p.ke) + ehead;
 
-  uint32_t st[8 * W];
+  uint32_t st[8 * C > 4 * W * T ? 8 * C : 4 * W * T];
   int st_exp = 0;
   const auto fetch = [&](int block0) {
-    const int block = min(block0 + mine, end - 1);
+    const int block = min(block0 + of, end - 1);
     const uint8_t* at = codes + (int64_t)block * BLK * HD;
     if (!values) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < T; ++t)
 #pragma unroll
         for (int c = 0; c < W; ++c) {
-          const u32x4 w = *(const u32x4*)(at + (t * 16 + r) * HD + c * 64 + q * 16);
+          const u32x4 w = *(const u32x4*)(at + ((part + t) * 16 + r) * HD + c * 64 + q * 16);
 #pragma unroll
           for (int j = 0; j < 4; ++j) st[(t * W + c) * 4 + j] = w[j];
         }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint8_t* row = at + ((j < 4 ? 4 * q + j : 12 + 4 * q + j)) * HD + (HD / 16) * r;
-        if constexpr (HD == 64) {
-          st[j] = *(const uint32_t*)row;
-        } else {
-          const u32x2 w = *(const u32x2*)row;
-          st[2 * j] = w[0];
-          st[2 * j + 1] = w[1];
-        }
-      }
+      for (int j = 0; j < 8; ++j) st[j] = *(const uint32_t*)(at + ((j < 4 ? 4 * q + j : 12 + 4 * q + j)) * HD + (HD / 16) * r + 4 * part);
     }
     st_exp = exps[block];
   };
   const auto convert = [&](int turn, int block0) {
     if (!values) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < T; ++t)
 #pragma unroll
         for (int c = 0; c < 2 * W; ++c)
-          frag[turn][mine][t * 2 * W + c][lane] = __builtin_bit_cast(u32x4, codes_bf16(st[t * 4 * W + 2 * c], st[t * 4 * W + 2 * c + 1]));
-      if (lane == 0) scale[turn][mine][0] = p.scale_log2 * kv8_pow2(st_exp - 127);
+          frag[turn][of][(part + t) * 2 * W + c][lane] = __builtin_bit_cast(u32x4, codes_bf16(st[t * 4 * W + 2 * c], st[t * 4 * W + 2 * c + 1]));
+      if (lane == 0) scale[turn][of][0] = p.scale_log2 * kv8_pow2(st_exp - 127);
     } else {
-      const int key0 = min(block0 + mine, end - 1) * BLK;
+      const int key0 = min(block0 + of, end - 1) * BLK;
       if (key0 + BLK > sq.len) {  // rows behind the last may hold anything
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (key0 + (j < 4 ? 4 * q + j : 12 + 4 * q + j) >= sq.len) {
-#pragma unroll
-            for (int c = 0; c < W; ++c) st[j * W + c] = 0;
-          }
+          if (key0 + (j < 4 ? 4 * q + j : 12 + 4 * q + j) >= sq.len) st[j] = 0;
       }
+      const uint32_t w0[4] = {st[0], st[1], st[2], st[3]}, w1[4] = {st[4], st[5], st[6], st[7]};
+      uint32_t t0[4], t1[4];
+      transpose4(w0, t0);
+      transpose4(w1, t1);
 #pragma unroll
-      for (int c = 0; c < W; ++c) {
-        const uint32_t w0[4] = {st[c], st[W + c], st[2 * W + c], st[3 * W + c]}, w1[4] = {st[4 * W + c], st[5 * W + c], st[6 * W + c], st[7 * W + c]};
-        uint32_t t0[4], t1[4];
-        transpose4(w0, t0);
-        transpose4(w1, t1);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) frag[turn][mine][KF + 4 * c + t][lane] = __builtin_bit_cast(u32x4, codes_f16(t0[t], t1[t]));
-      }
-      if (lane == 0) scale[turn][mine][1] = (float)(st_exp - 127);
+      for (int t = 0; t < 4; ++t) frag[turn][of][KF + 4 * part + t][lane] = __builtin_bit_cast(u32x4, codes_f16(t0[t], t1[t]));
+      if (lane == 0) scale[turn][of][1] = (float)(st_exp - 127);
     }
   };
 
   if (begin < end) {
     fetch(begin);
     convert(0, begin);
-    fetch(begin + 2);
+    fetch(begin + SB);
     __syncthreads();
     int turn = 0;
-    for (int block0 = begin; block0 < end; block0 += 2, turn ^= 1) {
-      if (block0 + 2 < end) {
-        convert(turn ^ 1, block0 + 2);
-        fetch(block0 + 4);
+    for (int block0 = begin; block0 < end; block0 += SB, turn ^= 1) {
+      if (block0 + SB < end) {
+        convert(turn ^ 1, block0 + SB);
+        fetch(block0 + 2 * SB);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < SB; ++i) {
         const int key0 = (block0 + i) * BLK;
         if (block0 + i >= end || key0 >= most) continue;  // (this wave's queries see none of it)
         const float ck = scale[turn][i][0], ev = scale[turn][i][1];
@@ -644,19 +667,20 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
     if (key + i < sq.len) out[i] = p.decay == 0.f ? w[i] : __builtin_fmaf(p.decay, out[i], w[i]);
 }
 
-// The weight that every row got from many columns.  A wave holds 64 keys as operands; the columns that see them pass by, 64 at a time through LDS.  Of a workgroup's four
-// waves two have the same keys, one for each half of the columns (workgroups of 128 keys: more of them, for the sake of balance).  The
-// scores are the attention kernel's again (the same products in the same order), exp2(score - lse) is their softmax.
+// The weight that every row got from many columns.  A wave holds 32 keys as operands (64 would leave registers for two waves per SIMD, and exponentials and
+// products of one wave follow each other: 201 us against 228 for 2 x 2048 queries over 6101 rows, 32 on 8 heads of 128); the columns that see them pass by, 64 at a time through LDS for the four waves.  Where that makes few workgroups the columns are shared out too (the first keys are
+// seen by all queries, the last by few: whole columns left 42 % of the CUs' time empty), and the shares added in their order afterwards.  The scores are the attention kernel's again (the same products in the same order), exp2(score - lse) is their softmax.
 template <int HD>
-__global__ __launch_bounds__(256, 2) void weights_kernel(Params p) {
-  constexpr int KT = 4, QF = HD / 32, COLS = 64, PIECES = COLS / 16 * QF * 64 / 256;  // key tiles; operands of a column tile; 16-byte pieces per thread
+__global__ __launch_bounds__(256, 4) void weights_kernel(Params p) {
+  constexpr int KT = 2, QF = HD / 32, COLS = 64;  // key tiles, operands of a column tile, columns on their way
   __shared__ u32x4 frag[2][COLS / 16 * QF][64];
   __shared__ float lses[2][COLS];
   __shared__ int lims[2][COLS];
-  __shared__ float other[2][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4, kvh = blockIdx.y, b = blockIdx.z, half = wave & 1;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
+  // (the first keys, which most queries see, first for all heads)
+  const int heads = p.kv_heads * p.batch, kvh = blockIdx.x % heads % p.kv_heads, b = blockIdx.x % heads / p.kv_heads, cs = blockIdx.y;
   const Seq sq = sequence(p, b);
-  const int wg_key0 = blockIdx.x * 32 * KT, key0 = wg_key0 + (wave >> 1) * 16 * KT;
+  const int wg_key0 = blockIdx.x / heads * 64 * KT, key0 = wg_key0 + wave * 16 * KT;
   if (wg_key0 >= sq.len) return;
   const int64_t head = (int64_t)sq.slot * p.slot_stride + (int64_t)kvh * p.ctx * HD;
   const int64_t ehead = (int64_t)sq.slot * p.exp_stride + (int64_t)kvh * (p.ctx / BLK);
@@ -676,43 +700,44 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(Params p) {
   const float* lse = p.lse + ((int64_t)b * p.kv_heads + kvh) * p.cols;
   const int n_cols = sq.rows * p.group;
   // queries from row wg_key0 on see something of these keys, those of the prefix if they begin within
-  const int begin = (wg_key0 < p.prefix ? 0 : min(max(wg_key0 - sq.pos0, 0), sq.rows)) * p.group;
+  const int from = (wg_key0 < p.prefix ? 0 : min(max(wg_key0 - sq.pos0, 0), sq.rows)) * p.group;
+  const int share = ((n_cols - from + COLS - 1) / COLS + p.col_splits - 1) / p.col_splits * COLS;  // of the columns, whole steps
+  const int begin = min(from + cs * share, n_cols), end = min(begin + share, n_cols);
 
-  u32x4 st[PIECES];
+  // wave w brings column tile w: every lane its 16-byte pieces of one column
+  u32x4 st[QF];
   float st_lse = INFINITY;
   int st_lim = 0;
+  const bf16_t* queries = p.q + (int64_t)b * p.q_bs + (int64_t)(kvh * p.group) * p.q_hs + q * 16;
   const auto fetch = [&](int c0) {
+    const int want = c0 + wave * 16 + r, col = min(want, n_cols - 1), t = query_of(p, col), g = col - t * p.group;  // (one that is none sees no key)
+    const bf16_t* at = queries + (int64_t)t * p.q_ts + (int64_t)g * p.q_hs;
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const int f = i * 4 + wave, c = f % QF, col = min(c0 + f / QF * 16 + r, n_cols - 1), t = query_of(p, col), g = col - t * p.group;
-      st[i] = *(const u32x4*)(p.q + (int64_t)b * p.q_bs + (int64_t)t * p.q_ts + (int64_t)(kvh * p.group + g) * p.q_hs + (c >> 1) * 64 + q * 16 + (c & 1) * 8);
-    }
-    const int col = c0 + lane;  // (one that is none: it sees no key)
-    st_lse = lse[min(col, n_cols - 1)];
-    st_lim = col < n_cols ? limit_of(p, sq, sq.pos0 + query_of(p, col)) : 0;
+    for (int c = 0; c < QF; ++c) st[c] = *(const u32x4*)(at + (c >> 1) * 64 + (c & 1) * 8);
+    st_lse = lse[col];
+    st_lim = want < n_cols ? limit_of(p, sq, sq.pos0 + t) : 0;
   };
   const auto put = [&](int turn) {
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) frag[turn][i * 4 + wave][lane] = st[i] ^ u32x4{p.q_sign, p.q_sign, p.q_sign, p.q_sign};
-    if (wave == 0) {
-      lses[turn][lane] = st_lse;
-      lims[turn][lane] = st_lim;
+    for (int c = 0; c < QF; ++c) frag[turn][wave * QF + c][lane] = st[c] ^ u32x4{p.q_sign, p.q_sign, p.q_sign, p.q_sign};
+    if (q == 0) {
+      lses[turn][wave * 16 + r] = st_lse;
+      lims[turn][wave * 16 + r] = st_lim;
     }
   };
-  if (begin < n_cols) {
+  if (begin < end) {
     fetch(begin);
     put(0);
     fetch(begin + COLS);
     __syncthreads();
     int turn = 0;
-    for (int c0 = begin; c0 < n_cols; c0 += COLS, turn ^= 1) {
-      if (c0 + COLS < n_cols) {
+    for (int c0 = begin; c0 < end; c0 += COLS, turn ^= 1) {
+      if (c0 + COLS < end) {
         put(turn ^ 1);
         fetch(c0 + 2 * COLS);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int ct = half * 2 + i;
+      for (int ct = 0; ct < COLS / 16; ++ct) {
         const float ls = lses[turn][ct * 16 + r];
         const int lim = lims[turn][ct * 16 + r];
         bf16x8 qf[1][QF];
@@ -735,7 +760,7 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(Params p) {
       __syncthreads();
     }
   }
-  // over the 16 columns of a tile, then over the two halves; lane 4 t + j of a group of 16 has key 16 t + 4 q + j
+  // over the 16 columns of a tile; lane 4 t + j of a group of 16 has key 16 t + 4 q + j
   float mine = 0.f;
 #pragma unroll
   for (int t = 0; t < KT; ++t)
@@ -746,14 +771,26 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(Params p) {
       for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o, 64);
       mine = r == 4 * t + j ? x : mine;
     }
-  if (half) other[wave >> 1][lane] = mine;
-  __syncthreads();
   const int key = key0 + (r >> 2) * 16 + 4 * q + (r & 3);
-  if (!half && key < sq.len) {
-    mine += other[wave >> 1][lane];
-    float* out = p.weights + ((int64_t)sq.slot * p.kv_heads + kvh) * p.ctx + key;
-    *out = p.decay == 0.f ? mine : __builtin_fmaf(p.decay, *out, mine);
+  if (r < 4 * KT && key < sq.len) {
+    if (p.col_splits > 1) {
+      p.wpart[(((int64_t)cs * p.batch + b) * p.kv_heads + kvh) * p.score_rows + key] = mine;
+    } else {
+      float* out = p.weights + ((int64_t)sq.slot * p.kv_heads + kvh) * p.ctx + key;
+      *out = p.decay == 0.f ? mine : __builtin_fmaf(p.decay, *out, mine);
+    }
   }
+}
+
+// The columns' shares of every row's weight together
+__global__ __launch_bounds__(256) void weights_sum_kernel(Params p) {
+  const int kvh = blockIdx.y, b = blockIdx.z, key = blockIdx.x * 256 + threadIdx.x;
+  const Seq sq = sequence(p, b);
+  if (key >= sq.len) return;
+  float x = 0.f;
+  for (int s = 0; s < p.col_splits; ++s) x += p.wpart[(((int64_t)s * p.batch + b) * p.kv_heads + kvh) * p.score_rows + key];
+  float* out = p.weights + ((int64_t)sq.slot * p.kv_heads + kvh) * p.ctx + key;
+  *out = p.decay == 0.f ? x : __builtin_fmaf(p.decay, *out, x);
 }
 
 constexpr int PROMPT_NT = 2;
@@ -765,7 +802,7 @@ constexpr int PROMPT_NT = 2;
 // and 13.3 / 17.1, 12 x 32 heads 14.0 / 13.7).
 struct Plan {
   bool decode;
-  int nt, waves, col_groups, splits, cols, score_rows;
+  int nt, waves, col_groups, splits, cols, score_rows, col_splits;
   size_t part, ml, lse, scores, bytes;
 };
 
@@ -788,7 +825,11 @@ Plan plan_of(const md_kv8_cache* c, const md_kv8_attn_args* a) {
   pl.lse = pl.ml + (pl.splits > 1 ? cols * pl.splits * 2 * 4 : 0);
   pl.scores = (pl.lse + (a->weights ? cols * 4 : 0) + 15) & ~(size_t)15;
   pl.score_rows = blocks * BLK;
-  pl.bytes = pl.scores + (a->weights && pl.decode ? (size_t)cols * pl.score_rows * 4 : 0);
+  const int64_t key_groups = (int64_t)((max_len + 127) / 128) * c->kv_heads * a->batch;
+  pl.col_splits = (int)std::max<int64_t>(1, std::min<int64_t>({(3072 + key_groups - 1) / key_groups, (pl.cols + 255) / 256, 16}));
+  pl.bytes = pl.scores;
+  if (a->weights && pl.decode) pl.bytes += (size_t)cols * pl.score_rows * 4;
+  if (a->weights && !pl.decode && pl.col_splits > 1) pl.bytes += (size_t)pl.col_splits * a->batch * c->kv_heads * pl.score_rows * 4;
   return pl;
 }
 
@@ -844,6 +885,10 @@ extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_at
   p.weights = a->weights;
   p.scores = a->weights && pl.decode ? (float*)(ws + pl.scores) : nullptr;
   p.score_rows = pl.score_rows;
+  p.wpart = (float*)(ws + pl.scores);
+  p.col_splits = pl.col_splits;
+  p.batch = a->batch;
+  p.by_length = p.max_len >= 2048 && a->batch > 1 && a->batch <= 64 && ((int64_t)p.max_len + a->q_len + 64 * PROMPT_NT) * p.group < 0x3fffffff;
   p.join_groups = pl.splits > 1 ? (pl.cols + 3) / 4 : 0;
   const int64_t groups = (int64_t)pl.col_groups * pl.splits, all = groups * cache->kv_heads * a->batch;
   MD_CHECK_ARG(all <= 0x7fffffff);
@@ -883,9 +928,12 @@ extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_at
     MD_TRY(md_launch_status());
   }
   if (a->weights && !pl.decode) {
-    const dim3 wg((p.max_len + 127) / 128, cache->kv_heads, a->batch);
+    const int64_t all_keys = (int64_t)((p.max_len + 127) / 128) * cache->kv_heads * a->batch;
+    MD_CHECK_ARG(all_keys <= 0x7fffffff);
+    const dim3 wg(all_keys, pl.col_splits);
     if (cache->head_dim == 64) hipLaunchKernelGGL(weights_kernel<64>, wg, block, 0, s, p);
     else hipLaunchKernelGGL(weights_kernel<128>, wg, block, 0, s, p);
+    if (pl.col_splits > 1) hipLaunchKernelGGL(weights_sum_kernel, dim3((p.max_len + 255) / 256, cache->kv_heads, a->batch), block, 0, s, p);
     MD_TRY(md_launch_status());
   }
   return MD_OK;

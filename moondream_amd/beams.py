@@ -58,8 +58,8 @@ def select_beams(logits: torch.Tensor, scores: torch.Tensor, ended: Optional[tor
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     at = tokens.data_ptr()
     a = _lib.MdBeamArgs(logits.data_ptr(), logits.stride(0), _DTYPES[logits.dtype], batch, beams, vocab, suppress_id, max(end_id, -1),
-                        _need(scores, "scores", torch.float32, dev, shape), None if ended is None else _need(ended, "ended", torch.int32, dev, shape),
-                        None if rank_weight is None else _need(rank_weight, "rank_weight", torch.float32, dev, shape),
+                        _need(scores, "scores", torch.float32, dev.index, shape), None if ended is None else _need(ended, "ended", torch.int32, dev.index, shape),
+                        None if rank_weight is None else _need(rank_weight, "rank_weight", torch.float32, dev.index, shape),
                         at, at + 4 * batch * beams, new.data_ptr(), at + 8 * batch * beams, ws.data_ptr(), need)
     _launch(dev.index, "md_beam_select", lib.md_beam_select, C.byref(a))
     return BeamChoice(tokens, parents, new, stop)
@@ -114,4 +114,4 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, into: 
         return
     dev = _gpu(parents, "reorder_states")
     _launch(dev.index, "md_state_reorder", _lib.load().md_state_reorder, (_lib.MdStatePart * len(parts))(*parts), len(parts),
-            _need(parents, "parents", torch.int32, dev, (batch, beams)), batch, beams)
+            _need(parents, "parents", torch.int32, dev.index, (batch, beams)), batch, beams)

@@ -39,10 +39,10 @@ def _launch(index: int, what: str, call, *args) -> None:
         _lib.check(status, what)
 
 
-def _need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, shape: tuple) -> int:
+def _need(t: torch.Tensor, name: str, dtype: torch.dtype, index: int, shape: tuple) -> int:
     """The address of a contiguous tensor that is what it has to be."""
-    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device}, wanted contiguous {shape} {dtype} on {device}")
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device}, wanted contiguous {shape} {dtype} on cuda:{index}")
     return t.data_ptr()
 
 
@@ -85,6 +85,7 @@ class BlockCache:
         self.slots, self.kv_heads, self.ctx, self.head_dim = slots, heads, ctx, dim
         self.device = torch.device("cuda", k.device.index if k.device.index is not None else torch.cuda.current_device())
         self._index = self.device.index
+        self._weight_shape = (slots, heads, ctx)
         self._lib = _lib.load()
         self._workspaces: dict = {}  # bytes that calls of a shape need
         stride = (k.stride(0), k_exp.stride(0)) if slots > 1 else (heads * ctx * dim, heads * ctx // BLOCK)
@@ -92,35 +93,36 @@ class BlockCache:
         self._ref = C.byref(self._struct)
 
     def _per_sequence(self, t: Optional[torch.Tensor], name: str, batch: int) -> Optional[int]:
-        return None if t is None else _need(t, name, _I32, self.device, (batch,))
+        return None if t is None else _need(t, name, _I32, self._index, (batch,))
 
     def _batch(self, batch: int, slot: Optional[torch.Tensor]) -> None:
         if batch <= 0 or (slot is None and batch > self.slots):
             raise ValueError(f"a batch of {batch} sequences in {self.slots} slots")
 
-    def _rows_of(self, t: torch.Tensor, name: str, heads: Optional[int]) -> tuple:
-        """The strides of bf16 rows that are as the kernels take them."""
-        if t.dim() != 4 or t.dtype != _BF16 or t.device != self.device or t.shape[3] != self.head_dim or (heads is not None and t.shape[2] != heads):
-            raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device}, wanted [batch, tokens, {heads or 'heads'}, {self.head_dim}] bfloat16 on {self.device}")
+    def _rows_of(self, t: torch.Tensor, name: str) -> tuple:
+        """The strides of bf16 rows [batch, tokens, heads, head_dim] that are as the kernels take them."""
         s = t.stride()
-        if t.data_ptr() % 16 or (s[0] | s[1] | s[2]) % 8 or s[3] != 1:
+        if len(s) != 4 or t.dtype is not _BF16 or t.get_device() != self._index or t.shape[3] != self.head_dim:
+            raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device}, wanted [batch, tokens, heads, {self.head_dim}] bfloat16 on {self.device}")
+        if s[3] != 1 or (s[0] | s[1] | s[2]) % 8 or t.data_ptr() % 16:
             raise ValueError(f"{name}: rows of head_dim have to be contiguous and 16-byte aligned (strides {s})")
         return s
 
     def append(self, k: torch.Tensor, v: torch.Tensor, row0: torch.Tensor, new: Optional[torch.Tensor] = None, slot: Optional[torch.Tensor] = None) -> None:
         """Rows row0[b] .. of every sequence from bf16 ``k``, ``v`` [batch, tokens, kv_heads, head_dim] (views of a projection's rows will do; keys
         rotated already); ``new``: how many of the tokens count, per sequence.  Rows past ``ctx`` are dropped.  A slot at most once."""
-        ks, vs = self._rows_of(k, "k", self.kv_heads), self._rows_of(v, "v", self.kv_heads)
-        batch, tokens = k.shape[:2]
-        if v.shape != k.shape:
-            raise ValueError(f"keys {tuple(k.shape)} and values {tuple(v.shape)}")
+        ks, vs = self._rows_of(k, "k"), self._rows_of(v, "v")
+        shape = k.shape
+        batch, tokens, heads, _ = shape
+        if v.shape != shape or heads != self.kv_heads:
+            raise ValueError(f"keys {tuple(shape)} and values {tuple(v.shape)}, wanted [batch, tokens, {self.kv_heads}, {self.head_dim}]")
         self._batch(batch, slot)
         if tokens == 0:
             return
         of = (batch,)
         _launch(self._index, "md_kv8_append", self._lib.md_kv8_append, self._ref, k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
-                None if slot is None else _need(slot, "slot", _I32, self.device, of), _need(row0, "row0", _I32, self.device, of),
-                None if new is None else _need(new, "new", _I32, self.device, of), batch, tokens)
+                None if slot is None else _need(slot, "slot", _I32, self._index, of), _need(row0, "row0", _I32, self._index, of),
+                None if new is None else _need(new, "new", _I32, self._index, of), batch, tokens)
 
     def read(self, row0: Optional[torch.Tensor], rows: int, kv_len: Optional[torch.Tensor] = None, slot: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """Rows row0[b] .. row0[b] + rows - 1 (None: from 0) as bf16 [batch, kv_heads, rows, head_dim] keys and values, exactly what the codes stand
@@ -137,7 +139,7 @@ class BlockCache:
         return k, v
 
     def _weights(self, w: Optional[torch.Tensor], name: str) -> Optional[int]:
-        return None if w is None else _need(w, name, _F32, self.device, (self.slots, self.kv_heads, self.ctx))
+        return None if w is None else _need(w, name, _F32, self._index, self._weight_shape)
 
     def attention(self, q: torch.Tensor, kv_len: torch.Tensor, q_pos0: Optional[torch.Tensor] = None, q_rows: Optional[torch.Tensor] = None,
                   slot: Optional[torch.Tensor] = None, prefix_len: int = 0, scale: Optional[float] = None, max_len: Optional[int] = None,
@@ -148,7 +150,7 @@ class BlockCache:
         ``prefix_len`` rows all of these.  ``q_rows``: how many of the queries count (the others' outputs stay as ``out`` has them; without
         ``out`` they are zeros).  ``max_len``: no sequence is longer (sizes the launch; longer ones are cut).  ``scale``: 1 / sqrt(head_dim).
         ``weights`` (fp32 [slots, kv_heads, ctx]) <- decay * weights + the softmax weight that every row got in this call."""
-        qs = self._rows_of(q, "q", None)
+        qs = self._rows_of(q, "q")
         batch, tokens, heads, dim = q.shape
         if heads == 0 or heads % self.kv_heads:
             raise ValueError(f"{heads} query heads over {self.kv_heads} key heads")
@@ -161,13 +163,13 @@ class BlockCache:
         else:
             if out.shape != q.shape:
                 raise ValueError(f"out: {tuple(out.shape)}, wanted {tuple(q.shape)}")
-            os = self._rows_of(out, "out", heads)
+            os = self._rows_of(out, "out")
         if tokens == 0:
             return out
         longest = 0 if max_len is None else min(max_len, self.ctx)
         a = _lib.MdKv8AttnArgs(q.data_ptr(), qs[0], qs[1], qs[2], out.data_ptr(), os[0], os[1], os[2], batch, heads, tokens,
                                self._per_sequence(slot, "slot", batch), self._per_sequence(q_pos0, "q_pos0", batch),
-                               self._per_sequence(q_rows, "q_rows", batch), _need(kv_len, "kv_len", _I32, self.device, (batch,)), longest,
+                               self._per_sequence(q_rows, "q_rows", batch), _need(kv_len, "kv_len", _I32, self._index, (batch,)), longest,
                                min(prefix_len, self.ctx), 1.0 / math.sqrt(dim) if scale is None else scale, decay, self._weights(weights, "weights"), None, 0)
         shape = (batch, heads, tokens, longest, weights is None)
         need = self._workspaces.get(shape)

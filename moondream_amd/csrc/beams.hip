@@ -14,8 +14,9 @@
 
 namespace {
 
-constexpr int PIECE = 8192;  // logits of a workgroup: 32 per thread
-constexpr int PER = PIECE / 256;
+// Logits of a thread; a workgroup's piece is 256 times as many.  32 keep the choice among the pieces short; where they make fewer workgroups than there
+// are CUs, the latency of a thread's work counts: 8.
+constexpr int MANY = 32, FEW = 8;
 constexpr int MAXB = MD_MAX_BEAMS;
 constexpr int ROOM = 128;    // logits of a wave that are put in order together
 constexpr float F32_MOST = 3.4028234663852886e38f;
@@ -50,11 +51,11 @@ __device__ __forceinline__ float logit<bf16_t>(bf16_t x) { return bf2f(x); }
 template <>
 __device__ __forceinline__ float logit<float>(float x) { return x; }
 
-template <typename T>
+template <typename T, int PER>
 __global__ __launch_bounds__(256) void part_kernel(const T* __restrict__ logits, int64_t ld, int vocab, int beams, int suppress_id,
                                                    const float* __restrict__ scores, const int32_t* __restrict__ ended, int pieces,
                                                    uint64_t* __restrict__ best, double* __restrict__ sums) {
-  constexpr int E = 16 / sizeof(T), N = PER / E;  // elements of a load, loads of a thread
+  constexpr int E = 16 / sizeof(T), N = PER / E, PIECE = 256 * PER;  // elements of a load, loads of a thread
   __shared__ uint64_t lists[4 * MAXB], found[4][ROOM];
   __shared__ float wmax[4];
   __shared__ double wsum[4];
@@ -275,7 +276,11 @@ __global__ __launch_bounds__(64 * MAXB) void choose_kernel(int beams, int pieces
   }
 }
 
-size_t pieces_of(int vocab) { return ((size_t)vocab + PIECE - 1) / PIECE; }
+int per_thread(int64_t rows, int vocab) { return rows * ((vocab + 256 * MANY - 1) / (256 * MANY)) >= 256 ? MANY : FEW; }
+size_t pieces_of(int64_t rows, int vocab) {
+  const size_t piece = 256 * per_thread(rows, vocab);
+  return ((size_t)vocab + piece - 1) / piece;
+}
 
 // ------------------------------------------------------------------------------------------------------------- states
 constexpr int MAX_PARTS = 32;  // of a launch (80 bytes each in its arguments)
@@ -352,26 +357,32 @@ bool part_ok(const md_state_part& s, int64_t slots) {
 
 extern "C" size_t md_beam_workspace_bytes(int32_t batch, int32_t beams, int32_t vocab) {
   if (batch <= 0 || beams < 2 || beams > MAXB || vocab <= 0) return 0;
-  return (size_t)batch * beams * pieces_of(vocab) * (beams * sizeof(uint64_t) + 2 * sizeof(double));
+  return (size_t)batch * beams * pieces_of((int64_t)batch * beams, vocab) * (beams * sizeof(uint64_t) + 2 * sizeof(double));
 }
 
 extern "C" md_status md_beam_select(const md_beam_args* a, void* stream) {
   MD_CHECK_ARG(a && a->logits && a->scores && a->tokens && a->parents && a->scores_out && a->batch > 0 && a->vocab > 0 && a->ld >= a->vocab);
   MD_CHECK_ARG(a->beams >= 2 && a->beams <= MAXB && (a->dtype == MD_DTYPE_BF16 || a->dtype == MD_DTYPE_F32) && (int64_t)a->batch * a->beams <= 65535);
   MD_CHECK_ARG(a->end_id < a->vocab && (a->end_id >= 0 || !a->ended) && ((uintptr_t)a->logits & (a->dtype == MD_DTYPE_F32 ? 3 : 1)) == 0);
-  const int pieces = (int)pieces_of(a->vocab), rows = a->batch * a->beams;
+  const int rows = a->batch * a->beams, pieces = (int)pieces_of(rows, a->vocab);
   if (!a->workspace || a->workspace_bytes < md_beam_workspace_bytes(a->batch, a->beams, a->vocab)) return MD_ERR_WORKSPACE;
   MD_CHECK_ARG(((uintptr_t)a->workspace & 15) == 0);
   uint64_t* best = (uint64_t*)a->workspace;
   double* sums = (double*)(best + (size_t)rows * pieces * a->beams);
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid(pieces, rows);
-  if (a->dtype == MD_DTYPE_BF16)
-    hipLaunchKernelGGL(part_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t*)a->logits, a->ld, a->vocab, a->beams, a->suppress_id, a->scores, a->ended,
-                       pieces, best, sums);
-  else
-    hipLaunchKernelGGL(part_kernel<float>, grid, dim3(256), 0, s, (const float*)a->logits, a->ld, a->vocab, a->beams, a->suppress_id, a->scores, a->ended,
-                       pieces, best, sums);
+#define MD_PART(T, PER)                                                                                                                            \
+  hipLaunchKernelGGL((part_kernel<T, PER>), grid, dim3(256), 0, s, (const T*)a->logits, a->ld, a->vocab, a->beams, a->suppress_id, a->scores,      \
+                     a->ended, pieces, best, sums)
+  const bool many = per_thread(rows, a->vocab) == MANY;
+  if (a->dtype == MD_DTYPE_BF16) {
+    if (many) MD_PART(bf16_t, MANY);
+    else MD_PART(bf16_t, FEW);
+  } else {
+    if (many) MD_PART(float, MANY);
+    else MD_PART(float, FEW);
+  }
+#undef MD_PART
   hipLaunchKernelGGL(choose_kernel, dim3(a->batch), dim3(64 * a->beams), 0, s, a->beams, pieces, a->end_id, a->scores, a->ended, a->rank_weight, best, sums,
                      a->tokens, a->parents, a->scores_out, a->ended_out);
   return md_launch_status();

@@ -5,8 +5,7 @@
 // logits gives them and the sum, and only beams x beams totals are ever compared.
 //   part_kernel    one workgroup per (beam, piece of the vocabulary): the piece in registers; each wave's largest logits, its maximum and its sum
 //                  of exponentials
-//   choose_kernel  one workgroup per input, one wave per beam: sums joined in 64 bits, the beam's candidates; totals, their order by counting
-//                  who is ahead
+//   choose_kernel  one workgroup per input, one wave per beam: sums joined in 64 bits, the pieces' lists merged, totals; then the beams' lists merged
 // Bound by the logits' bytes; with few rows by the two launches.
 #include "wave_ops.hpp"
 
@@ -18,6 +17,7 @@ namespace {
 // are CUs, the latency of a thread's work counts: 8.
 constexpr int MANY = 32, FEW = 8;
 constexpr int MAXB = MD_MAX_BEAMS;
+constexpr int LISTED = 7680;  // candidates of an input that choose_kernel has in LDS (30 pieces of 16 beams, 64 of up to 10)
 constexpr int ROOM = 128;    // logits of a wave that are put in order together
 constexpr float F32_MOST = 3.4028234663852886e38f;
 
@@ -189,12 +189,9 @@ __global__ __launch_bounds__(64 * MAXB) void choose_kernel(int beams, int pieces
                                                            const float* __restrict__ rank_weight, const uint64_t* __restrict__ best,
                                                            const double* __restrict__ sums, int32_t* __restrict__ tokens, int32_t* __restrict__ parents,
                                                            float* scores_out, int32_t* ended_out) {
+  __shared__ uint64_t listed[LISTED];
   __shared__ Ranked cand[MAXB * MAXB];
   __shared__ double totals[MAXB * MAXB];
-  __shared__ int counts[MAXB * MAXB + 1];  // of every candidate who is ahead; candidates
-  if ((int)threadIdx.x <= MAXB * MAXB) {
-    for (int i = threadIdx.x; i <= MAXB * MAXB; i += blockDim.x) counts[i] = 0;
-  }
   const int lane = threadIdx.x & 63, k = threadIdx.x >> 6, b = blockIdx.x, row0 = b * beams, n = beams * beams, row = row0 + k;
   const float score = scores[row], weight = rank_weight ? rank_weight[row] : 1.f;
   if (!goes_on(scores, ended, row)) {  // (an ended beam of a score: itself, and nothing else)
@@ -218,24 +215,24 @@ __global__ __launch_bounds__(64 * MAXB) void choose_kernel(int beams, int pieces
     }
     s = wave_sum_f64(s);
     const double norm = m + log(s);
-    // A piece's list is in falling order: lane i goes along piece i's, its next entry on its way.  (More than 64 pieces: 64 at a time, the largest so far
-    // as one more entry of each lane.)
-    for (int first = 0; first < pieces; first += 64) {
-      const int piece = first + lane;
-      const uint64_t* mine = list + (int64_t)min(piece, pieces - 1) * beams;
-      uint64_t head = piece < pieces ? mine[0] : 0, next = piece < pieces ? mine[1] : 0, got = 0;
-      int at = 1;
+    // A piece's list is in falling order: lane i goes along piece i's, in LDS.  (As many pieces at a time as have room, 64 at most, the largest so far as one
+    // more entry of each lane.)
+    const int room = min(64, LISTED / n);
+    uint64_t* mine = listed + k * room * beams;
+    for (int first = 0; first < pieces; first += room) {
+      const int here = min(room, pieces - first);
+      for (int i = lane; i < here * beams; i += 64) mine[i] = list[first * beams + i];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (a wave's LDS accesses run in order)
+      uint64_t head = lane < here ? mine[lane * beams] : 0, got = 0;
+      int at = lane * beams, last = at + beams - 1;
       for (int j = 0; j < beams; ++j) {
         const uint64_t w = wave_most_u64(head > carry ? head : carry);
         if (lane == j) got = w;
         if (carry == w) carry = 0;
-        if (head == w && w != 0) {
-          head = next;
-          ++at;
-          next = at < beams ? mine[at] : 0;
-        }
+        if (head == w && w != 0) head = at < last ? mine[++at] : 0;
       }
       carry = got;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     if (lane < beams) {
       const double total = carry ? (double)score + ((double)value_of(carry) - norm) : -INFINITY;
@@ -246,33 +243,37 @@ __global__ __launch_bounds__(64 * MAXB) void choose_kernel(int beams, int pieces
   }
   __syncthreads();
   // (every input of this input's beams has been read: what follows may overwrite scores and ended)
-  // thread (i, part): who of `part`'s share of the candidates is ahead of candidate i
-  const int parts = 64 / beams, i = (int)threadIdx.x % n, part = (int)threadIdx.x / n, parent = i / beams;
-  const Ranked me = cand[i];
-  const int was_ended = ended && ended[row0 + parent] != 0;
-  int ahead = 0;
-  for (int j = part; part < parts && j < n; j += parts) {
-    const int p = (j * (65536 / beams + 1)) >> 16;  // j / beams
-    const Ranked o = cand[j];
-    ahead += o.logit != 0 && (o.rank > me.rank || (o.rank == me.rank && (p < parent || (p == parent && o.logit > me.logit))));
+  // Every beam's list is in falling order: lane i of the first wave goes along beam i's; of equal ranks the lower beam's is taken.
+  if (k != 0) return;
+  const auto key_of = [](const Ranked& c) {  // doubles as whole numbers of the same order; 0: no candidate
+    const uint64_t u = __builtin_bit_cast(uint64_t, c.rank + 0.0);
+    return c.logit == 0 ? 0 : (u >> 63) ? ~u : u | (1ull << 63);
+  };
+  const bool there = lane < beams;
+  const int was_ended = there && ended ? ended[row0 + lane] : 0;
+  int at = lane * beams;
+  const int last = at + beams - 1;
+  Ranked me = there ? cand[at] : Ranked{-INFINITY, 0};
+  uint64_t key = key_of(me);
+  int live = 0;
+  for (; live < beams; ++live) {
+    const uint64_t w = wave_most_u64(key);
+    if (w == 0) break;
+    if (lane == __builtin_ctzll(__ballot(key == w))) {
+      const int token = (int)index_of(me.logit), to = row0 + live;
+      tokens[to] = token;
+      parents[to] = lane;
+      scores_out[to] = (float)totals[at];
+      if (ended_out) ended_out[to] = was_ended != 0 || token == end_id;
+      me = at < last ? cand[++at] : Ranked{-INFINITY, 0};
+      key = key_of(me);
+    }
   }
-  if (ahead) atomicAdd(&counts[i], ahead);
-  if (part == 0 && me.logit != 0) atomicAdd(&counts[MAXB * MAXB], 1);
-  __syncthreads();
-  ahead = counts[i];
-  const int live = counts[MAXB * MAXB];
-  if (part == 0 && me.logit != 0 && ahead < beams) {
-    const int token = (int)index_of(me.logit), at = row0 + ahead;
-    tokens[at] = token;
-    parents[at] = parent;
-    scores_out[at] = (float)totals[i];
-    if (ended_out) ended_out[at] = was_ended || token == end_id;
-  }
-  if (part == 0 && i < beams && i >= live) {
-    tokens[row0 + i] = end_id;
-    parents[row0 + i] = i;
-    scores_out[row0 + i] = -INFINITY;
-    if (ended_out) ended_out[row0 + i] = 1;
+  if (there && lane >= live) {
+    tokens[row0 + lane] = end_id;
+    parents[row0 + lane] = lane;
+    scores_out[row0 + lane] = -INFINITY;
+    if (ended_out) ended_out[row0 + lane] = 1;
   }
 }
 

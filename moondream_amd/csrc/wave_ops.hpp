@@ -28,15 +28,19 @@ __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
 
 __device__ __forceinline__ uint32_t lane_63(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
 
-__device__ __forceinline__ uint64_t wave_most_u64(uint64_t v) {
-#define MD_STEP(C, R)                                                                                                   \
-  {                                                                                                                     \
-    const uint64_t w = ((uint64_t)dpp<C, R>((uint32_t)(v >> 32), 0u) << 32) | dpp<C, R>((uint32_t)v, 0u);               \
-    v = w > v ? w : v;                                                                                                  \
-  }
+__device__ __forceinline__ uint32_t wave_most_u32(uint32_t v) {
+#define MD_STEP(C, R) v = max(v, dpp<C, R>(v, 0u));
   MD_DPP_STEPS(MD_STEP)
 #undef MD_STEP
-  return ((uint64_t)lane_63((uint32_t)(v >> 32)) << 32) | lane_63((uint32_t)v);
+  return lane_63(v);
+}
+// by the upper halves, which mostly differ; by the lower ones where they do not
+__device__ __forceinline__ uint64_t wave_most_u64(uint64_t v) {
+  const uint32_t hi = wave_most_u32((uint32_t)(v >> 32));
+  const bool mine = (uint32_t)(v >> 32) == hi;
+  const uint64_t who = __ballot(mine);
+  const uint32_t lo = who & (who - 1) ? wave_most_u32(mine ? (uint32_t)v : 0u) : (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, __builtin_ctzll(who));
+  return ((uint64_t)hi << 32) | lo;
 }
 
 __device__ __forceinline__ float wave_most_f32(float v) {

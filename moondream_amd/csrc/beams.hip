@@ -33,11 +33,9 @@ __device__ __forceinline__ float value_of(uint64_t c) {
 }
 __device__ __forceinline__ uint32_t index_of(uint64_t c) { return ~(uint32_t)c; }
 
-// exp(x), x <= 0, to an ulp or two of fp32: what the product x * log2(e) lost goes into the result
-__device__ __forceinline__ float exp_of(float x) {
-  const float a = x * 1.44269502f, lost = __builtin_fmaf(x, 1.44269502f, -a) + x * 1.92596299e-8f, e = __builtin_amdgcn_exp2f(a);
-  return a > -126.f ? __builtin_fmaf(e, lost * 0.693147182f, e) : 0.f;
-}
+// exp(x), x <= 0: the product's rounding is 2^-24 of its size, another one for each logit, so that sums of many are off by far less; terms whose
+// exponents are large, and off by more, are small
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
 
 // a beam that has continuations of its own
 __device__ __forceinline__ bool goes_on(const float* scores, const int32_t* ended, int row) {
@@ -64,24 +62,23 @@ __global__ __launch_bounds__(256) void part_kernel(const T* __restrict__ logits,
   if (threadIdx.x < 8) lists[min(4 * beams + (int)threadIdx.x, 4 * MAXB - 1)] = 0;  // (the count runs over whole eights)
   __syncthreads();
   const T* x = logits + (int64_t)row * ld;
-  const int base = piece * PIECE;
-  const bool aligned = ((uintptr_t)x & 15) == 0;
+  const int base = piece * PIECE - (int)(((uintptr_t)x & 15) / sizeof(T));  // (loads are aligned wherever the row begins: its first piece begins before it)
   float v[PER];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int at = base + (i * 256 + (int)threadIdx.x) * E;
-    if (aligned && at + E <= vocab) {
+    if (at >= 0 && at + E <= vocab) {
       const u32x4 w = *(const u32x4*)(x + at);
       const T* e = (const T*)&w;
 #pragma unroll
       for (int j = 0; j < E; ++j) v[i * E + j] = logit<T>(e[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < E; ++j) v[i * E + j] = at + j < vocab ? logit<T>(x[at + j]) : -INFINITY;
+      for (int j = 0; j < E; ++j) v[i * E + j] = at + j >= 0 && at + j < vocab ? logit<T>(x[at + j]) : -INFINITY;
     }
   }
   const auto id_of = [&](int i) { return base + ((i / E) * 256 + (int)threadIdx.x) * E + i % E; };
-  if ((unsigned)(suppress_id - base) < (unsigned)PIECE) {
+  if (suppress_id >= 0 && (unsigned)(suppress_id - base) < (unsigned)PIECE) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) v[i] = id_of(i) == suppress_id ? -INFINITY : v[i];
   }
@@ -280,7 +277,7 @@ __global__ __launch_bounds__(64 * MAXB) void choose_kernel(int beams, int pieces
 int per_thread(int64_t rows, int vocab) { return rows * ((vocab + 256 * MANY - 1) / (256 * MANY)) >= 256 ? MANY : FEW; }
 size_t pieces_of(int64_t rows, int vocab) {
   const size_t piece = 256 * per_thread(rows, vocab);
-  return ((size_t)vocab + piece - 1) / piece;
+  return ((size_t)vocab + 7 + piece - 1) / piece;  // (up to 7 places before a row's first logit)
 }
 
 // ------------------------------------------------------------------------------------------------------------- states

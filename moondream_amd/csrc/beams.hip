@@ -289,7 +289,7 @@ struct Part {
   int64_t src_slot, dst_slot, src_outer, dst_outer, src_seg, dst_seg;
   int32_t per_seg, segs;   // words of a run, runs of an outer index
   int32_t first, width;    // the part's first workgroup; bytes of a word
-  int64_t words;
+  uint32_t words;
 };
 struct Parts {
   Part p[MAX_PARTS];
@@ -297,12 +297,10 @@ struct Parts {
 };
 
 template <typename W, int B>
-__device__ __forceinline__ void move_words(const Part& p, int64_t first, const int32_t* __restrict__ parents, int beams, int64_t slot0) {
-  const int64_t w = first + threadIdx.x;
+__device__ __forceinline__ void move_words(const Part& p, uint32_t first, const int32_t* __restrict__ parents, int beams, int64_t slot0) {
+  const uint32_t w = first + threadIdx.x;
   if (w >= p.words) return;
-  const int64_t run = w / p.per_seg;
-  const int in = (int)(w - run * p.per_seg), seg = (int)(run % p.segs);
-  const int64_t outer = run / p.segs;
+  const uint32_t run = w / (uint32_t)p.per_seg, in = w - run * (uint32_t)p.per_seg, outer = run / (uint32_t)p.segs, seg = run - outer * (uint32_t)p.segs;
   const char* src = p.src + slot0 * p.src_slot + outer * p.src_outer + seg * p.src_seg + (int64_t)in * sizeof(W);
   char* dst = p.dst + slot0 * p.dst_slot + outer * p.dst_outer + seg * p.dst_seg + (int64_t)in * sizeof(W);
   const bool in_place = p.src == p.dst;
@@ -328,7 +326,8 @@ __global__ __launch_bounds__(256) void reorder_kernel(Parts parts, const int32_t
   int i = 0;
   while (i + 1 < parts.n && (int)blockIdx.x >= parts.p[i + 1].first) ++i;
   const Part& p = parts.p[i];
-  const int64_t slot0 = (int64_t)blockIdx.y * beams, first = (int64_t)((int)blockIdx.x - p.first) * 256;
+  const int64_t slot0 = (int64_t)blockIdx.y * beams;
+  const uint32_t first = (blockIdx.x - (uint32_t)p.first) * 256;
   if (p.width == 16) move_words<u32x4, B>(p, first, parents + slot0, beams, slot0);
   else if (p.width == 4) move_words<uint32_t, B>(p, first, parents + slot0, beams, slot0);
   else move_words<uint8_t, B>(p, first, parents + slot0, beams, slot0);
@@ -337,6 +336,17 @@ __global__ __launch_bounds__(256) void reorder_kernel(Parts parts, const int32_t
 int64_t extent(const md_state_part& s, bool src, int64_t slots) {
   const int64_t a = src ? s.src_slot_stride : s.dst_slot_stride, b = src ? s.src_outer_stride : s.dst_outer_stride, c = src ? s.src_seg_stride : s.dst_seg_stride;
   return (slots - 1) * a + (s.outer - 1) * b + (s.segs - 1) * c + s.seg_bytes;
+}
+
+// bytes that a thread moves at once, and how many such words a slot has
+int width_of(const md_state_part& s) {
+  const uint64_t all = (uint64_t)s.src | (uint64_t)s.dst | (uint64_t)s.src_slot_stride | (uint64_t)s.dst_slot_stride | (uint64_t)s.src_outer_stride |
+                       (uint64_t)s.dst_outer_stride | (uint64_t)s.src_seg_stride | (uint64_t)s.dst_seg_stride | (uint64_t)s.seg_bytes;
+  return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+}
+int64_t words_of(const md_state_part& s) {
+  const int64_t per = s.seg_bytes / width_of(s);
+  return per > 0x7fffffff ? per : (double)per * s.segs * s.outer > 4e9 ? (int64_t)4e9 : per * s.segs * s.outer;
 }
 
 bool part_ok(const md_state_part& s, int64_t slots) {
@@ -388,21 +398,18 @@ extern "C" md_status md_beam_select(const md_beam_args* a, void* stream) {
 
 extern "C" md_status md_state_reorder(const md_state_part* parts, int32_t n_parts, const int32_t* parents, int32_t batch, int32_t beams, void* stream) {
   MD_CHECK_ARG(parts && n_parts > 0 && parents && batch > 0 && batch <= 65535 && beams > 0 && beams <= MAXB);
-  for (int i = 0; i < n_parts; ++i) MD_CHECK_ARG(part_ok(parts[i], (int64_t)batch * beams));
+  for (int i = 0; i < n_parts; ++i) MD_CHECK_ARG(part_ok(parts[i], (int64_t)batch * beams) && words_of(parts[i]) <= 0x7fffff00);
   for (int done = 0; done < n_parts;) {
     Parts ps;
     ps.n = 0;
     int64_t groups = 0;
     for (; done < n_parts && ps.n < MAX_PARTS; ++done) {
       const md_state_part& s = parts[done];
-      const uint64_t all = (uint64_t)s.src | (uint64_t)s.dst | (uint64_t)s.src_slot_stride | (uint64_t)s.dst_slot_stride | (uint64_t)s.src_outer_stride |
-                           (uint64_t)s.dst_outer_stride | (uint64_t)s.src_seg_stride | (uint64_t)s.dst_seg_stride | (uint64_t)s.seg_bytes;
-      const int width = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
-      const int64_t per = s.seg_bytes / width, words = per * s.segs * s.outer, mine = (words + 255) / 256;
-      MD_CHECK_ARG(per <= 0x7fffffff && mine <= 0x7fffffff);
+      const int width = width_of(s);
+      const int64_t per = s.seg_bytes / width, words = words_of(s), mine = (words + 255) / 256;
       if (groups + mine > 0x7fffffff) break;
       ps.p[ps.n++] = {(const char*)s.src, (char*)s.dst, s.src_slot_stride, s.dst_slot_stride, s.src_outer_stride, s.dst_outer_stride, s.src_seg_stride,
-                      s.dst_seg_stride, (int32_t)per, s.segs, (int32_t)groups, width, words};
+                      s.dst_seg_stride, (int32_t)per, s.segs, (int32_t)groups, width, (uint32_t)words};
       groups += mine;
     }
     const dim3 grid((unsigned)groups, batch);

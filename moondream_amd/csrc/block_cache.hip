@@ -30,13 +30,13 @@ struct Rows {
 // One wave per (sequence, block that the new rows touch, K or V, head); heads next to one another, as a token's heads are in memory.
 template <int HD>
 __global__ __launch_bounds__(256) void append_kernel(Cache c, Rows k, Rows v, const int32_t* __restrict__ slot, const int32_t* __restrict__ row0,
-                                                     const int32_t* __restrict__ n_new, int q_len, int n_blocks, int64_t n_tasks) {
+                                                     const int32_t* __restrict__ n_new, int q_len, uint32_t n_blocks, uint32_t n_tasks) {
   constexpr int CPR = HD / 8, N = BLK * CPR / 64;  // chunks of 8 coordinates: per row, per lane
   const int lane = threadIdx.x & 63;
-  int64_t task = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  uint32_t task = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (task >= n_tasks) return;
-  const int h = (int)(task % c.heads);
-  task /= c.heads;
+  const int h = (int)(task % (uint32_t)c.heads);
+  task /= (uint32_t)c.heads;
   const int which = (int)(task & 1);
   task >>= 1;
   const int nb = (int)(task % n_blocks), b = (int)(task / n_blocks);
@@ -97,42 +97,42 @@ __global__ __launch_bounds__(256) void append_kernel(Cache c, Rows k, Rows v, co
   if (lane == 0) *ep = (uint8_t)(e + 127);
 }
 
-// 16 coordinates per thread: 16 bytes in, 32 out; blockIdx.y: K or V
+// 16 coordinates per thread: 16 bytes in, 32 out.  A workgroup belongs to one head's keys or values of one sequence, so that all but the row is the same
+// for its threads.
 template <int HD>
 __global__ __launch_bounds__(256) void read_kernel(Cache c, const int32_t* __restrict__ slot, const int32_t* __restrict__ row0,
-                                                   const int32_t* __restrict__ kv_len, int rows, int64_t n, bf16_t* __restrict__ ko,
+                                                   const int32_t* __restrict__ kv_len, int rows, uint32_t groups, bf16_t* __restrict__ ko,
                                                    bf16_t* __restrict__ vo) {
   constexpr int CPR = HD / 16;
-  const int which = blockIdx.y;
-  const uint8_t* codes = which ? c.v : c.k;
-  const uint8_t* exps = which ? c.ve : c.ke;
-  bf16_t* out = which ? vo : ko;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int ch = (int)(i % CPR);
-    int64_t t = i / CPR;
-    const int r = (int)(t % rows);
-    t /= rows;
-    const int h = (int)(t % c.heads), b = (int)(t / c.heads);
-    const int sl = slot ? slot[b] : b;
-    const int64_t row = (int64_t)(row0 ? row0[b] : 0) + r;
-    u32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-    if (sl >= 0 && sl < c.slots && row >= 0 && row < min(kv_len ? kv_len[b] : c.ctx, c.ctx)) {
-      const u32x4 w = *(const u32x4*)(codes + (int64_t)sl * c.slot_stride + ((int64_t)h * c.ctx + row) * HD + ch * 16);
-      const float s = kv8_pow2((int)exps[(int64_t)sl * c.exp_stride + (int64_t)h * (c.ctx / BLK) + row / BLK] - 127);
-      float f[4][4];
+  uint32_t id = blockIdx.x;
+  const uint32_t part = id % groups;
+  id /= groups;
+  const int h = (int)(id % (uint32_t)c.heads);
+  id /= (uint32_t)c.heads;
+  const int which = id & 1, b = (int)(id >> 1);
+  const int64_t i = (int64_t)part * blockDim.x + threadIdx.x;
+  const int r = (int)(i / CPR), ch = (int)(i % CPR);
+  if (r >= rows) return;
+  const int sl = slot ? slot[b] : b, n = min(kv_len ? kv_len[b] : c.ctx, c.ctx);
+  const int64_t row = (int64_t)(row0 ? row0[b] : 0) + r;
+  u32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+  if (sl >= 0 && sl < c.slots && row >= 0 && row < n) {
+    const u32x4 w = *(const u32x4*)((which ? c.v : c.k) + (int64_t)sl * c.slot_stride + ((int64_t)h * c.ctx + row) * HD + ch * 16);
+    const float s = kv8_pow2((int)(which ? c.ve : c.ke)[(int64_t)sl * c.exp_stride + (int64_t)h * (c.ctx / BLK) + row / BLK] - 127);
+    float f[4][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) kv8_unpack4(w[j], f[j]);
+    for (int j = 0; j < 4; ++j) kv8_unpack4(w[j], f[j]);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        lo[2 * j] = pack_bf16x2(f[j][0] * s, f[j][1] * s);
-        lo[2 * j + 1] = pack_bf16x2(f[j][2] * s, f[j][3] * s);
-        hi[2 * j] = pack_bf16x2(f[j + 2][0] * s, f[j + 2][1] * s);
-        hi[2 * j + 1] = pack_bf16x2(f[j + 2][2] * s, f[j + 2][3] * s);
-      }
+    for (int j = 0; j < 2; ++j) {
+      lo[2 * j] = pack_bf16x2(f[j][0] * s, f[j][1] * s);
+      lo[2 * j + 1] = pack_bf16x2(f[j][2] * s, f[j][3] * s);
+      hi[2 * j] = pack_bf16x2(f[j + 2][0] * s, f[j + 2][1] * s);
+      hi[2 * j + 1] = pack_bf16x2(f[j + 2][2] * s, f[j + 2][3] * s);
     }
-    *(u32x4*)(out + i * 16) = lo;
-    *(u32x4*)(out + i * 16 + 8) = hi;
   }
+  bf16_t* out = (which ? vo : ko) + (((int64_t)b * c.heads + h) * rows * CPR + i) * 16;
+  *(u32x4*)out = lo;
+  *(u32x4*)(out + 8) = hi;
 }
 
 // ---------------------------------------------------------------------------------------------------------------- eviction
@@ -209,20 +209,20 @@ __global__ __launch_bounds__(SEL) void select_kernel(const float* __restrict__ w
   if (one) load(0);
   uint32_t prefix = 0, mask = 0, want = keep;  // the key's leading digits, and how many of those that share them stay
   for (int shift = 32 - DIGIT;; shift = max(shift - DIGIT, 0)) {
-    for (int j = tid; j < APART * COPIES; j += SEL) hist[j] = 0;
+    const int copies = mask == 0 ? COPIES : 1;  // (later on few keys are left that share the leading digits)
+    for (int j = tid; j < APART * copies; j += SEL) hist[j] = 0;
     __syncthreads();
     for (int j0 = 0; j0 < len; j0 += HELD * SEL) {
       if (!one) load(j0);
 #pragma unroll
       for (int i = 0; i < HELD; ++i)
-        if (row_of(j0, i) < len && (key[i] & mask) == prefix) atomicAdd(&hist[((key[i] >> shift) & ((1 << DIGIT) - 1)) + (lane & (COPIES - 1)) * APART], 1u);
+        if (row_of(j0, i) < len && (key[i] & mask) == prefix) atomicAdd(&hist[((key[i] >> shift) & ((1 << DIGIT) - 1)) + (lane & (copies - 1)) * APART], 1u);
     }
     __syncthreads();
     // this thread's two digits, the larger first: how many keys lie above them
     const int d1 = (1 << DIGIT) - 1 - 2 * tid, d0 = d1 - 1;
     uint32_t n1 = 0, n0 = 0;
-#pragma unroll
-    for (int c = 0; c < COPIES; ++c) {
+    for (int c = 0; c < copies; ++c) {
       n1 += hist[d1 + c * APART];
       n0 += hist[d0 + c * APART];
     }
@@ -285,19 +285,19 @@ __global__ __launch_bounds__(SEL) void select_kernel(const float* __restrict__ w
 template <int HD, bool IN_PLACE>
 __global__ __launch_bounds__(IN_PLACE ? 1024 : 256) void gather_kernel(Cache from, Cache to, const float* weights, float* weights_out,
                                                                        const int32_t* __restrict__ slot, const int32_t* kv_len, int32_t* len_out,
-                                                                       const int32_t* __restrict__ kept, int keep, int n_blocks, int64_t n_tasks) {
+                                                                       const int32_t* __restrict__ kept, int keep, int n_blocks, uint32_t n_tasks) {
   constexpr int CPR = HD / 16, N = BLK * CPR / 64, WAVES = IN_PLACE ? 16 : 4;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t task = IN_PLACE ? blockIdx.x : (int64_t)blockIdx.x * WAVES + wave;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t task = IN_PLACE ? blockIdx.x : blockIdx.x * WAVES + wave;
   if (task >= n_tasks) return;
   int nb0 = wave;
   if constexpr (!IN_PLACE) {
-    nb0 = (int)(task % n_blocks);
-    task /= n_blocks;
+    nb0 = (int)(task % (uint32_t)n_blocks);
+    task /= (uint32_t)n_blocks;
   }
   const int which = (int)(task & 1);
   task >>= 1;
-  const int h = (int)(task % from.heads), b = (int)(task / from.heads);
+  const int h = (int)(task % (uint32_t)from.heads), b = (int)(task / (uint32_t)from.heads);
   const int sl = slot ? slot[b] : b;
   const bool there = sl >= 0 && sl < from.slots && sl < to.slots;
   if (which == 0 && h == 0 && nb0 == 0 && lane == 0) len_out[b] = there ? min(min(max(kv_len[b], 0), from.ctx), keep) : 0;
@@ -388,12 +388,12 @@ extern "C" md_status md_kv8_append(const md_kv8_cache* cache, const void* k, int
   MD_CHECK_ARG((((uintptr_t)k | (uintptr_t)v) & 15) == 0 && (k_bs | k_ts | k_hs | v_bs | v_ts | v_hs) % 8 == 0);
   const int n_blocks = (int)(((int64_t)std::min(q_len, cache->ctx) + 2 * BLK - 2) / BLK);  // wherever in a block the first row falls
   const int64_t tasks = (int64_t)batch * n_blocks * 2 * cache->kv_heads, groups = (tasks + 3) / 4;
-  MD_CHECK_ARG(groups <= 0x7fffffff);
+  MD_CHECK_ARG(tasks <= 0x7fffffff);
   const Rows rk{(const bf16_t*)k, k_bs, k_ts, k_hs}, rv{(const bf16_t*)v, v_bs, v_ts, v_hs};
   if (cache->head_dim == 64)
-    hipLaunchKernelGGL(append_kernel<64>, dim3(groups), dim3(256), 0, (hipStream_t)stream, device_cache(cache), rk, rv, slot, row0, n_new, q_len, n_blocks, tasks);
+    hipLaunchKernelGGL(append_kernel<64>, dim3(groups), dim3(256), 0, (hipStream_t)stream, device_cache(cache), rk, rv, slot, row0, n_new, q_len, (uint32_t)n_blocks, (uint32_t)tasks);
   else
-    hipLaunchKernelGGL(append_kernel<128>, dim3(groups), dim3(256), 0, (hipStream_t)stream, device_cache(cache), rk, rv, slot, row0, n_new, q_len, n_blocks, tasks);
+    hipLaunchKernelGGL(append_kernel<128>, dim3(groups), dim3(256), 0, (hipStream_t)stream, device_cache(cache), rk, rv, slot, row0, n_new, q_len, (uint32_t)n_blocks, (uint32_t)tasks);
   return md_launch_status();
 }
 
@@ -401,12 +401,15 @@ extern "C" md_status md_kv8_read(const md_kv8_cache* cache, const int32_t* slot,
                                  void* k_out, void* v_out, void* stream) {
   MD_CHECK_ARG(kv8_cache_ok(cache) && k_out && v_out && batch > 0 && rows > 0 && (slot || batch <= cache->slots));
   MD_CHECK_ARG((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0);
-  const int64_t n = (int64_t)batch * cache->kv_heads * rows * (cache->head_dim / 16);
-  const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, 256 * 32), 2);
+  const int64_t chunks = (int64_t)rows * (cache->head_dim / 16), threads = chunks <= 128 ? 128 : 256, groups = (chunks + threads - 1) / threads;
+  const int64_t all = groups * cache->kv_heads * 2 * batch;
+  MD_CHECK_ARG(all <= 0x7fffffff);
   if (cache->head_dim == 64)
-    hipLaunchKernelGGL(read_kernel<64>, grid, dim3(256), 0, (hipStream_t)stream, device_cache(cache), slot, row0, kv_len, rows, n, (bf16_t*)k_out, (bf16_t*)v_out);
+    hipLaunchKernelGGL(read_kernel<64>, dim3(all), dim3(threads), 0, (hipStream_t)stream, device_cache(cache), slot, row0, kv_len, rows, (uint32_t)groups,
+                       (bf16_t*)k_out, (bf16_t*)v_out);
   else
-    hipLaunchKernelGGL(read_kernel<128>, grid, dim3(256), 0, (hipStream_t)stream, device_cache(cache), slot, row0, kv_len, rows, n, (bf16_t*)k_out, (bf16_t*)v_out);
+    hipLaunchKernelGGL(read_kernel<128>, dim3(all), dim3(threads), 0, (hipStream_t)stream, device_cache(cache), slot, row0, kv_len, rows, (uint32_t)groups,
+                       (bf16_t*)k_out, (bf16_t*)v_out);
   return md_launch_status();
 }
 
@@ -424,6 +427,9 @@ extern "C" md_status md_kv8_evict(const md_kv8_cache* from, const md_kv8_cache* 
   } else {
     MD_CHECK_ARG(caches_apart(from, to) && (!a->weights_out || apart(a->weights, wn, a->weights_out, wm)));
   }
+  const int n_blocks = (a->keep + BLK - 1) / BLK;
+  const int64_t heads2 = (int64_t)a->batch * from->kv_heads * 2, tasks = in_place ? heads2 : heads2 * n_blocks, groups = in_place ? tasks : (tasks + 3) / 4;
+  MD_CHECK_ARG(tasks <= 0x7fffffff);
   hipStream_t s = (hipStream_t)stream;
 #define MD_SELECT(HELD, COPIES)                                                                                                                    \
   hipLaunchKernelGGL((select_kernel<HELD, COPIES>), dim3(from->kv_heads, a->batch), dim3(SEL), 0, s, a->weights, a->slot, a->kv_len, a->kept,      \
@@ -431,12 +437,9 @@ extern "C" md_status md_kv8_evict(const md_kv8_cache* from, const md_kv8_cache* 
   if (from->ctx <= 4 * SEL) MD_SELECT(4, 2);
   else MD_SELECT(32, 8);
 #undef MD_SELECT
-  const int n_blocks = (a->keep + BLK - 1) / BLK;
-  const int64_t heads2 = (int64_t)a->batch * from->kv_heads * 2, tasks = in_place ? heads2 : heads2 * n_blocks, groups = in_place ? tasks : (tasks + 3) / 4;
-  MD_CHECK_ARG(groups <= 0x7fffffff);
 #define MD_GATHER(HD, IP)                                                                                                                        \
   hipLaunchKernelGGL((gather_kernel<HD, IP>), dim3(groups), dim3(IP ? 1024 : 256), 0, s, device_cache(from), device_cache(to), a->weights,       \
-                     a->weights_out, a->slot, a->kv_len, a->len_out, a->kept, a->keep, n_blocks, tasks)
+                     a->weights_out, a->slot, a->kv_len, a->len_out, a->kept, a->keep, n_blocks, (uint32_t)tasks)
   if (from->head_dim == 64) {
     if (in_place) MD_GATHER(64, true);
     else MD_GATHER(64, false);

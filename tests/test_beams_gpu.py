@@ -59,6 +59,16 @@ def test_ties_go_to_the_lower_beam_and_token():
     assert select_beams(logits.cuda(), torch.zeros(2, 3).cuda()).tokens.tolist() == [[0, 1, 2]] * 2
 
 
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_many_pieces_and_many_rows(dtype):
+    g = torch.Generator().manual_seed(7)
+    check((torch.randn(4, 300007, generator=g) * 2).to(dtype), -torch.rand(2, 2, generator=g))  # more pieces than a wave has lanes
+    check((torch.randn(16, 300007, generator=g) * 2).to(dtype), -torch.rand(1, 16, generator=g))  # ... and than lists have room
+    logits = (torch.randn(256, 8200, generator=g) * 2).to(dtype)
+    logits[3], logits[17], logits[40:56] = 1.0, logits[17].round(), logits[40:56].clamp(max=2.0)  # more equal logits than are put in order together
+    check(logits, -torch.rand(16, 16, generator=g), suppress_id=8199)
+
+
 def test_what_is_no_number():
     g = torch.Generator().manual_seed(2)
     logits = torch.randn(8, 300, generator=g)

@@ -187,6 +187,47 @@ def test_positions_padding_and_absent_sequences(tokens, prefix):
     attend(c, k, v, q[:4], [100, 128, 77, 60], slot=[2, 0, 1, 3], prefix=prefix, q_rows=[1, tokens, 0, tokens], weights=True)
 
 
+@pytest.mark.parametrize("dim, kv_heads, group, tokens, ctx", [(64, 8, 1, 200, 2300), (128, 8, 2, 150, 2100), (64, 3, 5, 90, 2400), (64, 1, 130, 3, 2100)])
+def test_ragged_batches_of_long_prompts(dim, kv_heads, group, tokens, ctx):
+    """Workgroups in the order of their reach: sequences of every length, padded, absent and empty ones among them, prefixes; more heads in a group than columns in a workgroup."""
+    g = torch.Generator().manual_seed(ctx + dim)
+    c, k, v = filled(g, 6, ctx, kv_heads, dim)
+    q = torch.randn(7, tokens, kv_heads * group, dim, generator=g).to(BF16)
+    lens, slot = [ctx, 300, 0, tokens, ctx - 1, 1111, 700], [0, 1, 2, 5, 4, 3, 6]
+    rows = [tokens, 1, tokens, tokens // 2, tokens - 1, 0, tokens]
+    attend(c, k, v, q, lens, slot=slot, q_rows=rows, weights=True, decay=0.25)
+    attend(c, k, v, q, lens, slot=slot, q_rows=rows, prefix=600, q_pos0=[50, 0, 5, ctx, -10, 1000, 0])
+
+
+def test_more_sequences_than_a_wave_has_lanes():
+    g = torch.Generator().manual_seed(70)
+    c, k, v = filled(g, 3, 2080, 1, 64)
+    q = torch.randn(70, 40, 1, 64, generator=g).to(BF16)
+    attend(c, k, v, q, [2080 - 29 * i for i in range(70)], slot=[i % 3 for i in range(70)], q_rows=[40 - i % 5 for i in range(70)])
+
+
+@pytest.mark.parametrize("dim, group", [(64, 1), (64, 17), (128, 1), (128, 20)])
+@pytest.mark.parametrize("batch, kv_heads, length", [(1, 2, 700), (9, 16, 1200), (30, 10, 520)])
+def test_few_queries_over_short_caches_in_one_launch_and_in_two(dim, group, batch, kv_heads, length):
+    g = torch.Generator().manual_seed(batch + dim + group)
+    slots = min(batch, 4)
+    c, k, v = filled(g, slots, length, kv_heads, dim)
+    q = torch.randn(batch, 1, kv_heads * group, dim, generator=g).to(BF16)
+    slot, lens = [i % slots for i in range(batch)], [max(0, length - 37 * i) for i in range(batch)]
+    attend(c, k, v, q, lens, slot=slot)
+    if batch <= slots:
+        attend(c, k, v, q, lens, slot=slot, weights=True, decay=0.0)
+
+
+def test_negative_and_no_scale():
+    g = torch.Generator().manual_seed(2)
+    c, k, v = filled(g, 2, 100, 2, 64)
+    for tokens in (1, 40):
+        q = torch.randn(2, tokens, 2, 64, generator=g).to(BF16)
+        attend(c, k, v, q, [100, 61], scale=-0.2, weights=True)
+        attend(c, k, v, q, [100, 61], scale=0.0, weights=True)
+
+
 def test_strided_queries_and_outputs():
     g = torch.Generator().manual_seed(1)
     c, k, v = filled(g, 2, 64, 2, 64)
@@ -325,6 +366,29 @@ def test_what_stays_and_how(dim, in_place, ctx, lens, keep, first, recent):
             if not in_place:
                 assert torch.equal(t[s, :, m:], was[s, :, m:])
     assert torch.equal(to.k[4], before[0][4])  # a slot that no sequence has
+
+
+@pytest.mark.parametrize("ctx, keep", [(4096, 1000), (4128, 4000), (40000, 5000), (70016, 33000)])
+def test_rows_that_stay_of_long_caches(ctx, keep):
+    """Weights held in registers, in one portion and in several; many equal ones at the border."""
+    g = torch.Generator().manual_seed(keep)
+    c = BlockCache(2, ctx, 2, 64)
+    c.k.random_(0, 120)
+    c.v.random_(0, 120)
+    w = torch.exp(2 * torch.randn(2, 2, ctx, generator=g))
+    w[0, 1] = torch.randint(0, 50, (ctx,), generator=g).float()
+    w[1, 0, ::3] = 0.75
+    lens = [ctx, ctx - 1234]
+    buf = torch.zeros(2 * 2 * ctx + 1, device="cuda")  # an address that is no multiple of 16
+    gw = buf[1:].view(2, 2, ctx)
+    gw.copy_(w)
+    kept, n = c.evict(gw, ints(lens), keep, first=3, recent=50, into=BlockCache(2, keep, 2, 64))
+    for b in range(2):
+        for h in range(2):
+            x = w[b, h, : lens[b]].clone()
+            x[:3] = x[lens[b] - 50 :] = math.inf
+            best = torch.sort(x, descending=True, stable=True).indices[:keep].sort().values
+            assert torch.equal(kept[b, h, : len(best)].cpu().long(), best) and bool((kept[b, h, len(best) :] == -1).all())
 
 
 def test_eviction_in_place_is_the_same_as_into_another_cache():

@@ -136,11 +136,11 @@ __global__ __launch_bounds__(256) void read_kernel(Cache c, const int32_t* __res
 }
 
 // ---------------------------------------------------------------------------------------------------------------- eviction
-// weights as unsigned numbers of the same order; a NaN is the least, a row that has to stay the largest
+// weights as unsigned numbers of the same order; a NaN is the least (1; 0 is no row), a row that has to stay the largest
 __device__ __forceinline__ uint32_t rank_key(float w, bool stays) {
   const uint32_t u = __float_as_uint(w);
   const uint32_t key = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return stays ? 0xffffffffu : (w == w ? key : 0u);
+  return stays ? 0xffffffffu : (w == w ? key : 1u);
 }
 
 constexpr int SEL = 1024;   // threads of the selection
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(SEL) void select_kernel(const float* __restrict__ w
           if (j + e < ctx) x[e] = w[j + e];
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) key[i + e] = rank_key(x[e], j + e < first || j + e >= len - recent);
+      for (int e = 0; e < 4; ++e) key[i + e] = j + e < len ? rank_key(x[e], j + e < first || j + e >= len - recent) : 0u;
     }
   };
   const auto row_of = [&](int j0, int i) { return j0 + wave * (HELD * 64) + (i & ~3) * 64 + lane * 4 + (i & 3); };
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(SEL) void select_kernel(const float* __restrict__ w
       if (!one) load(j0);
 #pragma unroll
       for (int i = 0; i < HELD; ++i)
-        if (row_of(j0, i) < len && (key[i] & mask) == prefix) atomicAdd(&hist[((key[i] >> shift) & ((1 << DIGIT) - 1)) + (lane & (copies - 1)) * APART], 1u);
+        if (key[i] != 0 && (key[i] & mask) == prefix) atomicAdd(&hist[((key[i] >> shift) & ((1 << DIGIT) - 1)) + (lane & (copies - 1)) * APART], 1u);
     }
     __syncthreads();
     // this thread's two digits, the larger first: how many keys lie above them
@@ -249,19 +249,15 @@ __global__ __launch_bounds__(SEL) void select_kernel(const float* __restrict__ w
     // above in the low half, equal in the high one: 32768 at most
     uint32_t mine = 0;
 #pragma unroll
-    for (int i = 0; i < HELD; ++i)
-      if (row_of(j0, i) < len) mine += (key[i] > prefix ? 1u : 0u) + (key[i] == prefix ? 1u << 16 : 0u);
+    for (int i = 0; i < HELD; ++i) mine += (key[i] > prefix ? 1u : 0u) + (key[i] == prefix ? 1u << 16 : 0u);
     uint32_t all, before = scan_before(mine, part, all);
     before = __builtin_amdgcn_readfirstlane(before);  // of the wave's first lane: all earlier waves'
+#pragma unroll
     for (int i = 0; i < HELD; i += 4) {
       uint32_t quad[4], sum = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        quad[e] = 0;
-        uint32_t k = 0;
-#pragma unroll
-        for (int u = 0; u < HELD; u += 4) k = u == i ? key[u + e] : k;
-        if (row_of(j0, i + e) < len) quad[e] = (k > prefix ? 1u : 0u) + (k == prefix ? 1u << 16 : 0u);
+        quad[e] = (key[i + e] > prefix ? 1u : 0u) + (key[i + e] == prefix ? 1u << 16 : 0u);
         sum += quad[e];
       }
       const uint32_t s = wave_scan_u32(sum);

@@ -9,6 +9,7 @@ current stream of their tensors' device, allocate through torch only, never sync
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -65,10 +66,10 @@ def select_beams(logits: torch.Tensor, scores: torch.Tensor, ended: Optional[tor
     return BeamChoice(tokens, parents, new, stop)
 
 
-def _runs(t: torch.Tensor, slot_dim: int, name: str):
-    """(slot stride, outer count and stride, run count and stride, run length), in bytes, of a tensor's slots."""
-    size = t.element_size()
-    dims = [(n, s * size) for d, (n, s) in enumerate(zip(t.shape, t.stride())) if d != slot_dim and n > 1]
+@functools.lru_cache(maxsize=256)
+def _runs(shape: tuple, stride: tuple, size: int, slot_dim: int, name: str):
+    """(slot stride, outer count and stride, run count and stride, run length), in bytes, of the slots of a tensor of that layout."""
+    dims = [(n, s * size) for d, (n, s) in enumerate(zip(shape, stride)) if d != slot_dim and n > 1]
     length = size
     while dims and dims[-1][1] == length:
         length *= dims.pop()[0]
@@ -79,9 +80,9 @@ def _runs(t: torch.Tensor, slot_dim: int, name: str):
         else:
             joined.append((n, s))
     if len(joined) > 2:
-        raise ValueError(f"{name}: strides {t.stride()} leave more than two dimensions that lie apart")
+        raise ValueError(f"{name}: strides {stride} leave more than two dimensions that lie apart")
     outer, segs = ([(1, 0)] * 2 + joined)[-2:]
-    return t.stride(slot_dim) * size, outer, segs, length
+    return stride[slot_dim] * size, outer, segs, length
 
 
 def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, into: Optional[Sequence[torch.Tensor]] = None, slot_dim: int = 0) -> None:
@@ -97,18 +98,18 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, into: 
         raise ValueError(f"{len(states)} states into {len(into)}")
     parts = []
     for i, (src, dst) in enumerate(zip(states, into)):
-        name = f"state {i}"
-        if src.shape != dst.shape or src.dtype != dst.dtype or src.device != parents.device or dst.device != parents.device:
-            raise ValueError(f"{name}: {tuple(src.shape)} {src.dtype} on {src.device} into {tuple(dst.shape)} {dst.dtype} on {dst.device}")
-        if not -src.dim() <= slot_dim < src.dim() or src.shape[slot_dim] < batch * beams:
-            raise ValueError(f"{name}: {tuple(src.shape)} has fewer than {batch * beams} slots in dimension {slot_dim}")
+        name, shape, stride, size = f"state {i}", src.shape, src.stride(), src.element_size()
+        if shape != dst.shape or src.dtype is not dst.dtype or src.device != parents.device or dst.device != parents.device:
+            raise ValueError(f"{name}: {tuple(shape)} {src.dtype} on {src.device} into {tuple(dst.shape)} {dst.dtype} on {dst.device}")
+        n = len(shape)
+        if not -n <= slot_dim < n or shape[slot_dim] < batch * beams:
+            raise ValueError(f"{name}: {tuple(shape)} has fewer than {batch * beams} slots in dimension {slot_dim}")
         if src.numel() == 0:
             continue
-        at = slot_dim % src.dim()
-        a = _runs(src, at, name)
-        b = a if src.stride() == dst.stride() else _runs(dst, at, name)
+        a = _runs(tuple(shape), stride, size, slot_dim % n, name)
+        b = a if dst is src else _runs(tuple(shape), dst.stride(), size, slot_dim % n, name)
         if (a[1][0], a[2][0], a[3]) != (b[1][0], b[2][0], b[3]):
-            raise ValueError(f"{name}: strides {src.stride()} into {dst.stride()}")
+            raise ValueError(f"{name}: strides {stride} into {dst.stride()}")
         parts.append((src.data_ptr(), dst.data_ptr(), a[0], b[0], a[1][1], b[1][1], a[2][1], b[2][1], a[3], a[1][0], a[2][0]))
     if not parts:
         return

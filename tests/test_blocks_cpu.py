@@ -218,11 +218,14 @@ def test_python_entry_points_refuse_without_a_gpu():
 
 
 def test_runs_of_views():
+    def runs(t, slot_dim):
+        return _runs(tuple(t.shape), t.stride(), t.element_size(), slot_dim, "x")
+
     slab = torch.zeros(6, 4, 3, 40, 8)
-    assert _runs(slab, 1, "x") == (3 * 40 * 8 * 4, (1, 0), (6, 4 * 3 * 40 * 8 * 4), 3 * 40 * 8 * 4)
-    assert _runs(slab[:, :, :, 5:9], 1, "x") == (3 * 40 * 8 * 4, (6, 4 * 3 * 40 * 8 * 4), (3, 40 * 8 * 4), 4 * 8 * 4)
-    assert _runs(slab[0], 0, "x") == (3 * 40 * 8 * 4, (1, 0), (1, 0), 3 * 40 * 8 * 4)
-    assert _runs(torch.zeros(4, dtype=torch.uint8), 0, "x") == (1, (1, 0), (1, 0), 1)
+    assert runs(slab, 1) == (3 * 40 * 8 * 4, (1, 0), (6, 4 * 3 * 40 * 8 * 4), 3 * 40 * 8 * 4)
+    assert runs(slab[:, :, :, 5:9], 1) == (3 * 40 * 8 * 4, (6, 4 * 3 * 40 * 8 * 4), (3, 40 * 8 * 4), 4 * 8 * 4)
+    assert runs(slab[0], 0) == (3 * 40 * 8 * 4, (1, 0), (1, 0), 3 * 40 * 8 * 4)
+    assert runs(torch.zeros(4, dtype=torch.uint8), 0) == (1, (1, 0), (1, 0), 1)
 
 
 def test_the_oracle_rounds_as_torch_does():

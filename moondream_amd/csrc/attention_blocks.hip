@@ -793,13 +793,14 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(Params p) {
   *out = p.decay == 0.f ? x : __builtin_fmaf(p.decay, *out, x);
 }
 
-constexpr int PROMPT_NT = 2;
-
 // How a call is cut.  Up to 32 columns a wave's tiles would stand empty, and its keys are what there is to read: the waves of a workgroup share
 // them.  Splits: enough workgroups for 256 CUs of 4 workgroups each, none with less than 8 blocks (decode) or 16.  Where that would be a second launch
 // for little work, workgroups of 16 waves (8 where registers allow no more) take all keys of a head: one per CU at most, up to two blocks a wave,
 // eight where half of the CUs have one (us, one launch against two: 1 x 32 heads of 64, 800 keys 7.0 / 8.2, 2000 keys 9.5 / 8.3; 8 x 32 heads 7.9 / 10.3
 // and 13.3 / 17.1, 12 x 32 heads 14.0 / 13.7).
+// Prompts: 32 columns a wave, 16 where more would stand empty (up to 64 columns) or where workgroups are few and short, so that one's latency counts, about
+// a microsecond a block (us, 32 / 16 columns: 767 queries of 32 heads of 64 17.0 / 13.0, 2048 of 32 on 8 heads of 128 76 / 64, but 512 queries of 64 on 8 heads
+// of 128 over 8192 rows 177 / 210).
 struct Plan {
   bool decode;
   int nt, waves, col_groups, splits, cols, score_rows, col_splits;
@@ -810,10 +811,11 @@ Plan plan_of(const md_kv8_cache* c, const md_kv8_attn_args* a) {
   Plan pl;
   pl.cols = a->q_len * (a->n_heads / c->kv_heads);
   pl.decode = pl.cols <= 32;
-  pl.nt = pl.decode ? (pl.cols <= 16 ? 1 : 2) : PROMPT_NT;
+  const int max_len = a->max_len > 0 ? std::min(a->max_len, c->ctx) : c->ctx, blocks = (max_len + BLK - 1) / BLK;
+  if (pl.decode) pl.nt = pl.cols <= 16 ? 1 : 2;
+  else pl.nt = pl.cols <= 64 || (blocks <= 128 && (int64_t)((pl.cols + 127) / 128) * c->kv_heads * a->batch <= 512) ? 1 : 2;
   const int per = 16 * pl.nt * (pl.decode ? 1 : 4);
   pl.col_groups = (pl.cols + per - 1) / per;
-  const int max_len = a->max_len > 0 ? std::min(a->max_len, c->ctx) : c->ctx, blocks = (max_len + BLK - 1) / BLK;
   const int64_t groups = (int64_t)pl.col_groups * c->kv_heads * a->batch;
   const int wide = pl.nt == 1 && c->head_dim == 64 ? 16 : 8;
   pl.waves = pl.decode && groups <= 256 && blocks >= 16 && blocks <= (groups >= 128 ? 8 : 2) * wide ? wide : 4;
@@ -888,7 +890,7 @@ extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_at
   p.wpart = (float*)(ws + pl.scores);
   p.col_splits = pl.col_splits;
   p.batch = a->batch;
-  p.by_length = p.max_len >= 2048 && a->batch > 1 && a->batch <= 64 && ((int64_t)p.max_len + a->q_len + 64 * PROMPT_NT) * p.group < 0x3fffffff;
+  p.by_length = p.max_len >= 2048 && a->batch > 1 && a->batch <= 64 && ((int64_t)p.max_len + a->q_len + 128) * p.group < 0x3fffffff;
   p.join_groups = pl.splits > 1 ? (pl.cols + 3) / 4 : 0;
   const int64_t groups = (int64_t)pl.col_groups * pl.splits, all = groups * cache->kv_heads * a->batch;
   MD_CHECK_ARG(all <= 0x7fffffff);
@@ -915,9 +917,11 @@ extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_at
     }
 #undef MD_DECODE
   } else if (cache->head_dim == 64) {
-    hipLaunchKernelGGL((prompt_kernel<64, PROMPT_NT>), dim3(all), block, 0, s, p);
+    if (pl.nt == 1) hipLaunchKernelGGL((prompt_kernel<64, 1>), dim3(all), block, 0, s, p);
+    else hipLaunchKernelGGL((prompt_kernel<64, 2>), dim3(all), block, 0, s, p);
   } else {
-    hipLaunchKernelGGL((prompt_kernel<128, PROMPT_NT>), dim3(all), block, 0, s, p);
+    if (pl.nt == 1) hipLaunchKernelGGL((prompt_kernel<128, 1>), dim3(all), block, 0, s, p);
+    else hipLaunchKernelGGL((prompt_kernel<128, 2>), dim3(all), block, 0, s, p);
   }
   MD_TRY(md_launch_status());
   const int tail = p.join_groups + (p.scores ? (p.max_len + 1023) / 1024 : 0);

@@ -6,7 +6,9 @@
 //   part_kernel    one workgroup per (beam, piece of the vocabulary): the piece in registers; each wave's largest logits, its maximum and its sum
 //                  of exponentials
 //   choose_kernel  one workgroup per input, one wave per beam: sums joined in 64 bits, the pieces' lists merged, totals; then the beams' lists merged
-// Bound by the logits' bytes; with few rows by the two launches.
+// Four beams of 51200 logits: 6.2 + 5.2 us, two launches' latency; 64 rows of 51200 bf16 logits 11.4 + 5.8 us; 64 rows of 131075 fp32 ones 21 us (1.6 TB/s: the
+// vector instructions, some 1000 for a wave's 2048 logits, follow the loads, as all workgroups run at once) and 13.6 us for 16 beams.
+// States move at 6.8 TB/s (16 x 4 beams, 1.6 GB in 235 us).
 #include "wave_ops.hpp"
 
 #include <algorithm>

@@ -2,7 +2,9 @@
 //
 // A block is 32 rows of one head.  One wave quantises a block: its largest magnitude gives the power of two, every lane holds 8 (append)
 // or 16 (evict) neighbouring coordinates of a few rows, and any lane may hold any row, because the block has ONE scale; so every
-// memory instruction of the wave covers whole rows, one after another.  All three are bound by memory.
+// memory instruction of the wave covers whole rows, one after another.  All three are bound by memory: 12000 new rows of 32 heads of 64 in 36 us
+// (4.1 TB/s) and back in 34 us (4.3 TB/s), 4096 of 32749 rows of 8 x 8 heads of 128 gathered in 33 us (4.0 TB/s).  A single row per sequence is
+// latency: 64 sequences in 5.4 us.
 #include "block_cache.hpp"
 #include "wave_ops.hpp"
 

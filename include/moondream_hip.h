@@ -885,12 +885,15 @@ md_status md_kv8_read(const md_kv8_cache* cache, const int32_t* slot, const int3
  * (query head h reads head h / (n_heads / kv_heads)).  q, o: bf16, element (b, t, h, d) at b * bs + t * ts + h * hs + d, 16-byte aligned,
  * strides % 8 == 0.  Query t of sequence b stands at row p = q_pos0[b] + t (q_pos0 NULL: the last q_rows[b] rows, kv_len[b] - q_rows[b] + t)
  * and sees the rows j <= p, with p < prefix_len all j < prefix_len, in every case j < kv_len[b] only; one that sees no row gives zeros.
- * Queries t >= q_rows[b] (NULL: q_len) are padding: their outputs stay as they are.
+ * Queries t >= q_rows[b] (NULL: q_len) are padding: their outputs stay as they are.  o may be q itself where no weights are wanted; else no element of
+ * o is one of q.
  * max_len bounds kv_len (longer ones count as max_len; 0: ctx) and sizes the launch.
  * weights (fp32 [slots][kv_heads][ctx], or NULL): weights[row] = decay * weights[row] + the sum over the sequence's queries and the
  * group's heads of the softmax weight that the row got, for the rows below kv_len; decay 0 does not read what was there.  With
  * weights a slot may appear once in a call.
- * Scores, softmax statistics, outputs and weights are held in fp32; a key's softmax weight enters the product with the values as fp16. */
+ * Scores, softmax statistics, outputs and weights are held in fp32; a key's softmax weight enters the product with the values as fp16.  The order of
+ * all sums follows from the counts of the call (not from the data): the same call gives the same bits.
+ * q_len * (n_heads / kv_heads)^2 < 2^32, q_len * (n_heads / kv_heads) < 2^23, batch and kv_heads < 2^16. */
 typedef struct {
   const void* q;
   int64_t q_bs, q_ts, q_hs;
@@ -917,7 +920,7 @@ md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_attn_args* ar
  * one that shares no memory with it, of as many heads, the same head_dim and ctx >= keep.
  * weights: fp32 [slots][kv_heads][ctx] of `from`; weights_out: the same of `to` (NULL: not wanted; in place: weights itself).
  * kept (int32 [batch][kv_heads][keep]): the rows that stayed, -1 behind the last;  len_out[b] = min(kv_len[b], keep), may be kv_len.
- * A slot may appear once in a call.  first + recent <= keep. */
+ * A slot may appear once in a call; one outside either cache is an absent sequence.  first + recent <= keep. */
 typedef struct {
   const float* weights;
   float* weights_out;
@@ -937,8 +940,8 @@ md_status md_kv8_evict(const md_kv8_cache* from, const md_kv8_cache* to, const m
  *   total(k, t) = scores[b][k] + logits[t] - log sum_v exp(logits[v])      of a beam that goes on (logits[suppress_id] = -inf)
  *   total(k, end_id) = scores[b][k], no other token                        of a beam that has ended (ended[b][k] != 0)
  * The `beams` largest total * rank_weight[b][k] (fp32, > 0; NULL: 1) are taken, in falling order; ties: the lower beam, then the larger logit,
- * then the lower token.  A beam whose score is -inf or NaN has no continuations, nor has a total of -inf (how a search begins: all
- * scores but the first -inf).  Sums and totals are taken in 64 bits.  NaN logits count as -inf, +inf as the largest float.
+ * then the lower token.  A beam whose score is -inf or NaN has no continuations, nor is a total (or a weighted one) of -inf or NaN one (how a
+ * search begins: all scores but the first -inf).  Sums and totals are taken in 64 bits.  NaN logits count as -inf, +inf as the largest float.
  *   tokens, parents [batch][beams]: the token, and the beam (of the same input) that it goes on from
  *   scores_out: its total;  ended_out: its beam had ended or the token is end_id.  May be scores / ended.
  * Where fewer continuations are left: token end_id, parent the place itself, score -inf, ended.

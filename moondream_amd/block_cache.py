@@ -128,7 +128,7 @@ class BlockCache:
         """Rows row0[b] .. row0[b] + rows - 1 (None: from 0) as bf16 [batch, kv_heads, rows, head_dim] keys and values, exactly what the codes stand
         for; zeros for rows outside [0, kv_len[b])."""
         given = next((t for t in (row0, kv_len, slot) if t is not None), None)
-        batch = self.slots if given is None else given.shape[0]
+        batch = self.slots if given is None else given.numel()
         self._batch(batch, slot)
         if rows < 0:
             raise ValueError(f"{rows} rows")
@@ -147,7 +147,7 @@ class BlockCache:
         """Softmax attention of ``q`` [batch, tokens, heads, head_dim] (bf16) over the first ``kv_len[b]`` rows; returns the same shape.
 
         A sequence's queries are its last rows unless ``q_pos0`` says where the first one stands; each sees the rows up to its own, those in the first
-        ``prefix_len`` rows all of these.  ``q_rows``: how many of the queries count (the others' outputs stay as ``out`` has them; without
+        ``prefix_len`` rows all of these.  ``out`` may be ``q`` itself where no weights are wanted.  ``q_rows``: how many of the queries count (the others' outputs stay as ``out`` has them; without
         ``out`` they are zeros).  ``max_len``: no sequence is longer (sizes the launch; longer ones are cut).  ``scale``: 1 / sqrt(head_dim).
         ``weights`` (fp32 [slots, kv_heads, ctx]) <- decay * weights + the softmax weight that every row got in this call."""
         qs = self._rows_of(q, "q")
@@ -194,7 +194,7 @@ class BlockCache:
             raise ValueError("into_weights without into: in place the weights move within themselves")
         if not (0 < keep <= to.ctx) or first < 0 or recent < 0 or first + recent > keep:
             raise ValueError(f"keep {keep}, first {first}, recent {recent}: wanted first + recent <= keep <= {to.ctx}")
-        batch = kv_len.shape[0]
+        batch = kv_len.numel()
         self._batch(batch, slot)
         to._batch(batch, slot)
         w = self._weights(weights, "weights")

@@ -855,6 +855,7 @@ extern "C" size_t md_kv8_attention_workspace_bytes(const md_kv8_cache* cache, co
 extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_attn_args* a, void* stream) {
   MD_CHECK_ARG(args_ok(cache, a) && a->q && a->o && a->kv_len && a->prefix_len >= 0);
   MD_CHECK_ARG((((uintptr_t)a->q | (uintptr_t)a->o) & 15) == 0 && (a->q_bs | a->q_ts | a->q_hs | a->o_bs | a->o_ts | a->o_hs) % 8 == 0);
+  MD_CHECK_ARG(!a->weights || a->o != (void*)a->q);  // (the weights are made from the queries again)
   MD_CHECK_ARG(a->scale > -INFINITY && a->scale < INFINITY && (!a->weights || (a->decay >= 0.f && a->decay < INFINITY)));
   const Plan pl = plan_of(cache, a);
   if (pl.bytes && (!a->workspace || a->workspace_bytes < pl.bytes)) return MD_ERR_WORKSPACE;

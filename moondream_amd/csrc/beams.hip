@@ -195,8 +195,9 @@ __global__ __launch_bounds__(64 * MAXB) void choose_kernel(int beams, int pieces
   const float score = scores[row], weight = rank_weight ? rank_weight[row] : 1.f;
   if (!goes_on(scores, ended, row)) {  // (an ended beam of a score: itself, and nothing else)
     if (lane < beams) {
-      const bool itself = lane == 0 && score > -INFINITY;
-      cand[k * beams + lane] = {itself ? (double)score * (double)weight : -INFINITY, itself ? candidate(0.f, end_id) : 0};
+      const double rank = (double)score * (double)weight;
+      const bool itself = lane == 0 && score > -INFINITY && rank > -INFINITY;
+      cand[k * beams + lane] = {itself ? rank : -INFINITY, itself ? candidate(0.f, end_id) : 0};
       totals[k * beams + lane] = itself ? (double)score : -INFINITY;
     }
   } else {
@@ -235,8 +236,9 @@ __global__ __launch_bounds__(64 * MAXB) void choose_kernel(int beams, int pieces
     }
     if (lane < beams) {
       const double total = carry ? (double)score + ((double)value_of(carry) - norm) : -INFINITY;
-      const bool real = total > -INFINITY;
-      cand[k * beams + lane] = {real ? total * (double)weight : -INFINITY, real ? carry : 0};
+      const double rank = total * (double)weight;
+      const bool real = total > -INFINITY && rank > -INFINITY;
+      cand[k * beams + lane] = {real ? rank : -INFINITY, real ? carry : 0};
       totals[k * beams + lane] = real ? total : -INFINITY;
     }
   }

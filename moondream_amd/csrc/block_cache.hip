@@ -431,7 +431,7 @@ extern "C" md_status md_kv8_evict(const md_kv8_cache* from, const md_kv8_cache* 
   hipStream_t s = (hipStream_t)stream;
 #define MD_SELECT(HELD, COPIES)                                                                                                                    \
   hipLaunchKernelGGL((select_kernel<HELD, COPIES>), dim3(from->kv_heads, a->batch), dim3(SEL), 0, s, a->weights, a->slot, a->kv_len, a->kept,      \
-                     from->slots, from->ctx, from->kv_heads, a->keep, a->first, a->recent)
+                     std::min(from->slots, to->slots), from->ctx, from->kv_heads, a->keep, a->first, a->recent)
   if (from->ctx <= 4 * SEL) MD_SELECT(4, 2);
   else MD_SELECT(32, 8);
 #undef MD_SELECT

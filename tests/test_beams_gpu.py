@@ -81,6 +81,12 @@ def test_what_is_no_number():
     scores = torch.tensor([[-1.0, -2.0, -3.0, -30.0], [-1.0, math.nan, -math.inf, -2.0]])
     check(logits, scores)
     check(logits, scores, ended=torch.tensor([[0, 0, 1, 0], [0, 1, 1, 0]], dtype=I32), end_id=3)
+    weight = torch.tensor([[1.0, 1.0, math.nan, 0.5], [math.inf, 1.0, 1.0, 1.0]])  # beams whose weighted totals are no numbers have no continuations
+    got = select_beams(logits.cuda(), scores.cuda(), rank_weight=weight.cuda(), end_id=3)
+    alive = scores.clone()
+    alive[0, 2] = alive[1, 0] = -math.inf
+    for a, b in zip(got, select_beams(logits.cuda(), alive.cuda(), rank_weight=torch.nan_to_num(weight, 1.0, 1.0).cuda(), end_id=3)):
+        assert torch.equal(a, b)
     dead = torch.full((1, 3), -math.inf)
     got = select_beams(logits[:3].cuda(), dead.cuda(), end_id=9)
     assert got.tokens.tolist() == [[9] * 3] and got.parents.tolist() == [[0, 1, 2]] and got.ended.tolist() == [[1] * 3] and bool((got.scores == -math.inf).all())

@@ -58,7 +58,7 @@ def test_append_and_read_refuse():
 
 
 def attention_args(**kw):
-    a = _lib.MdKv8AttnArgs(AT, 256, 128, 64, AT, 256, 128, 64, 2, 4, 1, None, None, None, AT, 0, 0, 0.125, 1.0, None, None, 0)
+    a = _lib.MdKv8AttnArgs(AT, 256, 128, 64, AT + 5 * GB, 256, 128, 64, 2, 4, 1, None, None, None, AT, 0, 0, 0.125, 1.0, None, None, 0)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -66,7 +66,7 @@ def attention_args(**kw):
 
 @pytest.mark.parametrize("bad", [dict(q=None), dict(o=None), dict(kv_len=None), dict(batch=0), dict(batch=5), dict(batch=70000, slot=AT), dict(q_len=0), dict(q_len=1 << 23),
                                  dict(n_heads=0), dict(n_heads=3), dict(max_len=-1), dict(prefix_len=-1), dict(q_ts=4), dict(o_hs=68), dict(q=AT + 4), dict(scale=math.nan),
-                                 dict(scale=math.inf), dict(weights=AT, decay=-1.0), dict(weights=AT, decay=math.inf), dict(weights=AT, decay=math.nan)], ids=str)
+                                 dict(scale=math.inf), dict(weights=AT, decay=-1.0), dict(weights=AT, decay=math.inf), dict(weights=AT, decay=math.nan), dict(weights=AT, o=AT), dict(n_heads=1 << 18, q_len=16)], ids=str)
 def test_attention_refuses(bad):
     assert _lib.load().md_kv8_attention(C.byref(cache()), C.byref(attention_args(workspace=AT, workspace_bytes=GB, **bad)), None) == 1
 

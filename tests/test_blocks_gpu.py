@@ -236,7 +236,10 @@ def test_strided_queries_and_outputs():
     full = torch.zeros(2, 4, 3, 64, dtype=BF16, device="cuda")
     out = full.transpose(1, 2)
     assert c.attention(q, ints([50, 64]), out=out) is out
-    assert torch.equal(out.contiguous(), c.attention(q.contiguous(), ints([50, 64])))
+    want = c.attention(q.contiguous(), ints([50, 64]))
+    assert torch.equal(out.contiguous(), want)
+    again = q.contiguous()
+    assert c.attention(again, ints([50, 64]), out=again) is again and torch.equal(again, want)  # in the queries' place
 
 
 @pytest.mark.parametrize("dim, kv_heads, group, tokens, length", [(64, 2, 1, 1, 5003), (64, 1, 8, 1, 9001), (128, 1, 4, 1, 7777), (128, 2, 2, 40, 4001), (64, 1, 1, 500, 3011)])
@@ -409,6 +412,8 @@ def test_eviction_of_absent_sequences_touches_nothing():
     c, _, _ = filled(g, 2, 64, 1, 64)
     w = torch.rand(2, 1, 64, device="cuda")
     before = c.k.clone(), w.clone()
+    kept, n = c.evict(w, ints([64, 64]), 8, slot=ints([1, 5]), into=BlockCache(1, 64, 1, 64))  # a slot that the other cache does not have
+    assert n.tolist() == [0, 0] and bool((kept == -1).all())
     kept, n = c.evict(w, ints([64, 64]), 8, slot=ints([-1, 2]))
     assert n.tolist() == [0, 0] and bool((kept == -1).all()) and torch.equal(before[0], c.k) and torch.equal(before[1], w)
 

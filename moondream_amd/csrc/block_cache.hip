@@ -168,7 +168,7 @@ __device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* part, uint
 
 // One workgroup per (head, sequence): the keep-th largest key digit by digit (a histogram in LDS each), then the rows in their order: those above
 // it, and as many of its equals, lowest first, as are still wanted.  Up to HELD * 1024 rows are read once and stay in registers, longer caches
-// come by portion by portion in every pass.  Of a portion a wave has HELD * 64 rows in a row, of these a lane four in a row, 256 apart.  COPIES of the
+// come by portion by portion in every pass.  Of a portion a wave has HELD * 64 rows in a row, a lane every 64th.  COPIES of the
 // histogram lie in different banks, so that lanes that count the same digit (the first digit is sign, exponent and two bits: few are in use) mostly
 // do so in different places.  Caches of up to 4096 rows take HELD 4, COPIES 2: 801 rows of 32 heads in 8 us against 25 with 32 and 8.
 template <int HELD, int COPIES>
@@ -188,25 +188,18 @@ __global__ __launch_bounds__(SEL) void select_kernel(const float* __restrict__ w
     return;
   }
   const float* w = weights + ((int64_t)sl * heads + h) * ctx;
-  const bool quads = ((uintptr_t)w & 15) == 0;  // (ctx % 32 == 0: all heads' or none's)
   uint32_t key[HELD];
+  const auto row_of = [&](int j0, int i) { return j0 + wave * (HELD * 64) + i * 64 + lane; };
   const auto load = [&](int j0) {
+    float x[HELD];
 #pragma unroll
-    for (int i = 0; i < HELD; i += 4) {
-      const int j = j0 + wave * (HELD * 64) + i * 64 + lane * 4;
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
-      if (j + 3 < ctx && quads) {
-        x = *(const f32x4*)(w + j);
-      } else {
+    for (int i = 0; i < HELD; ++i) x[i] = w[min(row_of(j0, i), len - 1)];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (j + e < ctx) x[e] = w[j + e];
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) key[i + e] = j + e < len ? rank_key(x[e], j + e < first || j + e >= len - recent) : 0u;
+    for (int i = 0; i < HELD; ++i) {
+      const int j = row_of(j0, i);
+      key[i] = j < len ? rank_key(x[i], j < first || j >= len - recent) : 0u;
     }
   };
-  const auto row_of = [&](int j0, int i) { return j0 + wave * (HELD * 64) + (i & ~3) * 64 + lane * 4 + (i & 3); };
   const bool one = len <= HELD * SEL;
   if (one) load(0);
   uint32_t prefix = 0, mask = 0, want = keep;  // the key's leading digits, and how many of those that share them stay
@@ -254,23 +247,17 @@ __global__ __launch_bounds__(SEL) void select_kernel(const float* __restrict__ w
     for (int i = 0; i < HELD; ++i) mine += (key[i] > prefix ? 1u : 0u) + (key[i] == prefix ? 1u << 16 : 0u);
     uint32_t all, before = scan_before(mine, part, all);
     before = __builtin_amdgcn_readfirstlane(before);  // of the wave's first lane: all earlier waves'
+    uint32_t na = n_above + (before & 0xffffu), ne = n_equal + (before >> 16);
 #pragma unroll
-    for (int i = 0; i < HELD; i += 4) {
-      uint32_t quad[4], sum = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        quad[e] = (key[i + e] > prefix ? 1u : 0u) + (key[i + e] == prefix ? 1u << 16 : 0u);
-        sum += quad[e];
-      }
-      const uint32_t s = wave_scan_u32(sum);
-      uint32_t at = before + s - sum;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t eq = n_equal + (at >> 16), place = n_above + (at & 0xffffu) + min(eq, want);
-        if (quad[e] == 1u || (quad[e] != 0 && eq < want)) out[place] = row_of(j0, i + e);
-        at += quad[e];
-      }
-      before += lane_63(s);
+    for (int i = 0; i < HELD; ++i) {
+      asm("" : "+v"(key[i]));  // (the comparisons are made again: 64 masks kept from above would be spilled)
+      const bool above = key[i] > prefix, equal = key[i] == prefix;
+      const uint64_t a = __ballot(above), e = __ballot(equal);
+      const uint32_t eq = ne + __builtin_amdgcn_mbcnt_hi((uint32_t)(e >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)e, 0u));
+      const uint32_t place = na + __builtin_amdgcn_mbcnt_hi((uint32_t)(a >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)a, 0u)) + min(eq, want);
+      if (above || (equal && eq < want)) out[place] = row_of(j0, i);
+      na += __popcll(a);
+      ne += __popcll(e);
     }
     n_above += all & 0xffffu;
     n_equal += all >> 16;

@@ -833,7 +833,7 @@ Plan plan_of(const md_kv8_cache* c, const md_kv8_attn_args* a) {
   pl.scores = (pl.lse + (a->weights ? cols * 4 : 0) + 15) & ~(size_t)15;
   pl.score_rows = blocks * BLK;
   const int64_t key_groups = (int64_t)((max_len + 127) / 128) * c->kv_heads * a->batch;
-  pl.col_splits = (int)std::max<int64_t>(1, std::min<int64_t>({(3072 + key_groups - 1) / key_groups, (pl.cols + 255) / 256, 16}));
+  pl.col_splits = (int)std::max<int64_t>(1, std::min<int64_t>({(3000 + key_groups - 1) / key_groups, (pl.cols + 255) / 256, 16}));
   pl.bytes = pl.scores;
   if (a->weights && pl.decode) pl.bytes += (size_t)cols * pl.score_rows * 4;
   if (a->weights && !pl.decode && pl.col_splits > 1) pl.bytes += (size_t)pl.col_splits * a->batch * c->kv_heads * pl.score_rows * 4;

@@ -6,6 +6,7 @@ import torch
 
 from moondream_amd.beams import reorder_states, select_beams
 from moondream_amd.block_cache import BlockCache
+from moondream_amd.engine import no_collection
 
 import blocks_util as U
 
@@ -157,6 +158,48 @@ def test_states_past_32_bits():
         x[i, :64] = 10 + i
     reorder_states([x], torch.tensor([[3, 0, 2, 1]], dtype=I32, device="cuda"))
     assert x[:, -1].tolist() == [4, 1, 3, 2] and x[:, 0].tolist() == [13, 10, 12, 11] and not bool(x[:, 64:-64:4097].any())
+
+
+def test_captured_calls_replay_and_streams_do_not_disturb_one_another():
+    """A portion of prompts with weights, a choice and a reordering in two graphs over the same inputs, replayed in turn, between eager runs and beside work on another stream."""
+    g = torch.Generator().manual_seed(21)
+    cache = BlockCache(4, 640, 2, 64)
+    rows = torch.randn(4, 640, 2, 64, generator=g).to(BF16).cuda()
+    cache.append(rows, rows.flip(1), torch.zeros(4, dtype=I32, device="cuda"))
+    q, length = torch.randn(4, 300, 4, 64, generator=g).to(BF16).cuda(), torch.tensor([640, 500, 301, 640], dtype=I32, device="cuda")
+    logits, scores = torch.randn(8, 9000, generator=g).cuda(), -torch.rand(2, 4, generator=g).cuda()
+    state = torch.randn(3, 8, 2, 40, generator=g).cuda()
+
+    def work(w, into):
+        o = cache.attention(q, length, weights=w, decay=0.0)
+        choice = select_beams(logits, scores, end_id=5)
+        reorder_states([state], choice.parents, into=[into], slot_dim=1)
+        return (o, *choice)
+
+    buffers = [(torch.zeros(4, 2, 640, device="cuda"), torch.zeros_like(state)) for _ in range(4)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work(*buffers[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    with no_collection():
+        for i in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                outs.append(work(*buffers[i]))
+            graphs.append(graph)
+    for turn in range(4):
+        for t in (q, logits, state):
+            t.copy_(torch.randn(t.shape, generator=g).to(t.dtype))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            beside = work(*buffers[3])
+        graphs[turn % 2].replay()
+        eager = work(*buffers[2])
+        torch.cuda.synchronize()
+        for a, b, c in zip((*outs[turn % 2], *buffers[turn % 2]), (*eager, *buffers[2]), (*beside, *buffers[3])):
+            assert torch.equal(a, b) and torch.equal(c, b), f"turn {turn}"
 
 
 @pytest.mark.parametrize("beams, dim, group", [(4, 64, 1), (3, 128, 4)])

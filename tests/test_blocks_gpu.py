@@ -325,6 +325,40 @@ def test_offsets_past_32_bits():
                 assert torch.equal(now[h, b0 : b0 + 32].cpu().double(), U.e4m3(was[h, b0 : b0 + 32] * 2.0**-e) * 2.0**e)
 
 
+def test_one_head_past_32_bits():
+    """A single head whose keys take over 4 GiB; the last rows outweigh the 67 million zeros before them."""
+    ctx, n = (1 << 26) + 96, 70
+    c = BlockCache(1, ctx, 1, 64)
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(1, n, 1, 64, generator=g)
+    x[..., 0] = 16.0
+    x = x.to(BF16).cuda()
+    c.append(x, x.flip(1), ints([ctx - n]))
+    k, v = (r[0].cpu().double() for r in c.read(ints([ctx - n]), n))
+    w = torch.zeros(1, 1, ctx, device="cuda")
+    for tokens in (1, 40):
+        q = torch.randn(1, tokens, 1, 64, generator=g)
+        q[..., 0] = 24.0
+        q = q.to(BF16)
+        got = c.attention(q.cuda(), ints([ctx]), weights=w, decay=0.0).cpu().double()
+        t = q[0, :, 0].double() @ k[0].T / 8
+        seen = torch.arange(n)[None] <= torch.arange(n - tokens, n)[:, None]
+        e = torch.where(seen, torch.exp(t), 0.0)
+        zeros = ctx - n
+        p = e / (e.sum(1, keepdim=True) + zeros)
+        o, size = p @ v[0], p @ v[0].abs()
+        mass = float((q[0, :, 0].double().abs() @ k[0].abs().T / 8).max())
+        tol = U.attention_tolerance(o, size, float(t.abs().max()), mass, 64, n, float(v.abs().max())) + size * 2.0**-20
+        assert bool(((got[0, :, 0] - o).abs() <= tol).all())
+        near = (w[0, 0, ctx - n :].cpu().double() - p.sum(0)).abs()
+        assert bool((near <= U.weights_tolerance(p.sum(0), float(t.abs().max()), mass, 64, tokens) + p.sum(0) * 2.0**-20).all())
+    into, into_w = BlockCache(1, 96, 1, 64), torch.zeros(1, 1, 96, device="cuda")
+    kept, length = c.evict(w, ints([ctx]), 64, recent=1, into=into, into_weights=into_w)
+    best = torch.sort(w[0, 0, ctx - n : ctx - 1].cpu(), descending=True, stable=True).indices[:63]
+    rows = torch.cat([best.sort().values, torch.tensor([n - 1])]) + ctx - n
+    assert torch.equal(kept[0, 0].cpu().long(), rows) and length.tolist() == [64] and torch.equal(into_w[0, 0, :64].cpu(), w[0, 0].cpu()[rows])
+
+
 # ------------------------------------------------------------------------------------------------------------------------- eviction
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("in_place", [False, True])

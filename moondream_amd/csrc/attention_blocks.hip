@@ -25,6 +25,7 @@
 #include "wave_ops.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -608,23 +609,29 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
     const int col = blockIdx.x * 4 + wave;
     if (col >= n_cols) return;
     const int64_t c0 = bh * p.cols + col;
-    float m, l, o[N] = {};
-    const float f = join_factor(p.part_ml + c0 * p.splits * 2, p.splits, lane, m, l);
+    float m, l, f, o[N] = {};
     const float* part = p.part + c0 * p.splits * HD + lane * N;
-    for (int s = 0; s < p.splits; s += 8) {
-      float x[8][N];
+    const auto add = [&](int s, auto many) {  // splits s .. s + U - 1, requested together
+      constexpr int U = decltype(many)::value;
+      float x[U][N];
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < N; ++i) x[u][i] = part[(int64_t)min(s + u, p.splits - 1) * HD + i];
+      if (s == 0) f = join_factor(p.part_ml + c0 * p.splits * 2, p.splits, lane, m, l);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
+      for (int u = 0; u < U; ++u) {
         const float fu = s + u < p.splits ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s + u)) : 0.f;
         if (s + u < p.splits) {
 #pragma unroll
           for (int i = 0; i < N; ++i) o[i] = __builtin_fmaf(x[u][i], fu, o[i]);
         }
       }
+    };
+    if (p.splits <= 8) {
+      add(0, std::integral_constant<int, 8>());
+    } else {
+      for (int s = 0; s < p.splits; s += 16) add(s, std::integral_constant<int, 16>());
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int t = query_of(p, col), g = col - t * p.group;

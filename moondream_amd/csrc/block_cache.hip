@@ -140,7 +140,7 @@ __global__ __launch_bounds__(256) void read_kernel(Cache c, const int32_t* __res
 // ---------------------------------------------------------------------------------------------------------------- eviction
 // weights as unsigned numbers of the same order; a NaN is the least (1; 0 is no row), a row that has to stay the largest
 __device__ __forceinline__ uint32_t rank_key(float w, bool stays) {
-  const uint32_t u = __float_as_uint(w);
+  const uint32_t u = __float_as_uint(w + 0.f);  // (-0 and 0 are equal)
   const uint32_t key = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
   return stays ? 0xffffffffu : (w == w ? key : 1u);
 }

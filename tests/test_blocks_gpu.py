@@ -428,6 +428,18 @@ def test_rows_that_stay_of_long_caches(ctx, keep):
             assert torch.equal(kept[b, h, : len(best)].cpu().long(), best) and bool((kept[b, h, len(best) :] == -1).all())
 
 
+@pytest.mark.parametrize("ctx", [96, 8192])
+def test_zeros_of_both_signs_are_equal_weights(ctx):
+    c = BlockCache(1, ctx, 1, 64)
+    w = torch.zeros(1, 1, ctx)
+    w[0, 0, 1::2] = 0.0
+    w[0, 0, ::2] = -0.0
+    w[0, 0, 40] = -1e-30
+    w[0, 0, 50] = 1e-45
+    kept, n = c.evict(w.cuda(), ints([ctx]), 45)
+    assert kept[0, 0].tolist() == [j for j in range(45) if j != 40] + [50] and n.tolist() == [45]
+
+
 def test_eviction_in_place_is_the_same_as_into_another_cache():
     g = torch.Generator().manual_seed(11)
     c, k, v = filled(g, 2, 6000, 2, 64, spread=2.0)

@@ -871,7 +871,8 @@ typedef struct {
 
 /* Rows row0[b] .. row0[b] + n_new[b] - 1 of every sequence (n_new NULL: q_len) from bf16 keys and values, element (b, t, h, d) at
  * b * bs + t * ts + h * hs + d, 16-byte aligned, strides % 8 == 0.  Rows past ctx are dropped.  A block that began before row0 keeps at
- * least its scale; where the new rows need a larger one its older rows are rounded to that.  Other rows stay as they are. */
+ * least its scale; where the new rows need a larger one its older rows are rounded to that.  The new rows are the sequence's last: rows behind
+ * them in their last block count as gone (their codes stay, under the block's new scale).  All other blocks stay as they are. */
 md_status md_kv8_append(const md_kv8_cache* cache, const void* k, int64_t k_bs, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_bs,
                         int64_t v_ts, int64_t v_hs, const int32_t* slot, const int32_t* row0, const int32_t* n_new, int32_t batch,
                         int32_t q_len, void* stream);

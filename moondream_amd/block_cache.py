@@ -23,14 +23,12 @@ from . import _lib
 
 BLOCK = _lib.MD_KV8_BLOCK
 _BF16, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
-
-
-_current_device, _raw_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
+_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _launch(index: int, what: str, call, *args) -> None:
     """An entry point on the current stream of device ``index``, which is made the current one if it is not."""
-    if _current_device() == index:
+    if _device() == index:  # (there are tensors on a device: torch has been set up)
         status = call(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -110,7 +108,8 @@ class BlockCache:
 
     def append(self, k: torch.Tensor, v: torch.Tensor, row0: torch.Tensor, new: Optional[torch.Tensor] = None, slot: Optional[torch.Tensor] = None) -> None:
         """Rows row0[b] .. of every sequence from bf16 ``k``, ``v`` [batch, tokens, kv_heads, head_dim] (views of a projection's rows will do; keys
-        rotated already); ``new``: how many of the tokens count, per sequence.  Rows past ``ctx`` are dropped.  A slot at most once."""
+        rotated already); ``new``: how many of the tokens count, per sequence.  Rows past ``ctx`` are dropped.  The new rows are the sequence's last (what lay behind
+        them in their last block is gone).  A slot at most once."""
         ks, vs = self._rows_of(k, "k"), self._rows_of(v, "v")
         shape = k.shape
         batch, tokens, heads, _ = shape
@@ -164,6 +163,8 @@ class BlockCache:
             if out.shape != q.shape:
                 raise ValueError(f"out: {tuple(out.shape)}, wanted {tuple(q.shape)}")
             os = self._rows_of(out, "out")
+            if 0 in os:  # (an expanded dimension: outputs would be written over one another)
+                raise ValueError(f"out: strides {os}")
         if tokens == 0:
             return out
         longest = 0 if max_len is None else min(max_len, self.ctx)
@@ -174,6 +175,8 @@ class BlockCache:
         shape = (batch, heads, tokens, longest, weights is None)
         need = self._workspaces.get(shape)
         if need is None:
+            if len(self._workspaces) >= 1024:  # (max_len may be another in every step)
+                self._workspaces.clear()
             need = self._workspaces[shape] = self._lib.md_kv8_attention_workspace_bytes(self._ref, C.byref(a))
         if need:
             ws = torch.empty(need, dtype=_U8, device=self.device)

@@ -906,7 +906,8 @@ extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_at
   p.by_length = p.max_len >= 2048 && a->batch > 1 && a->batch <= 64 && ((int64_t)p.max_len + a->q_len + 128) * p.group < 0x3fffffff;
   p.join_groups = pl.splits > 1 ? (pl.cols + 3) / 4 : 0;
   const int64_t groups = (int64_t)pl.col_groups * pl.splits, all = groups * cache->kv_heads * a->batch;
-  MD_CHECK_ARG(all <= 0x7fffffff);
+  const int64_t key_groups = (int64_t)((p.max_len + 127) / 128) * cache->kv_heads * a->batch;
+  MD_CHECK_ARG((pl.decode || all <= MOST_GROUPS) && (pl.decode || !a->weights || key_groups <= MOST_GROUPS));
   const dim3 grid(groups, cache->kv_heads, a->batch), block(256);
   hipStream_t s = (hipStream_t)stream;
   if (pl.decode) {
@@ -945,9 +946,7 @@ extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_at
     MD_TRY(md_launch_status());
   }
   if (a->weights && !pl.decode) {
-    const int64_t all_keys = (int64_t)((p.max_len + 127) / 128) * cache->kv_heads * a->batch;
-    MD_CHECK_ARG(all_keys <= 0x7fffffff);
-    const dim3 wg(all_keys, pl.col_splits);
+    const dim3 wg(key_groups, pl.col_splits);
     if (cache->head_dim == 64) hipLaunchKernelGGL(weights_kernel<64>, wg, block, 0, s, p);
     else hipLaunchKernelGGL(weights_kernel<128>, wg, block, 0, s, p);
     if (pl.col_splits > 1) hipLaunchKernelGGL(weights_sum_kernel, dim3((p.max_len + 255) / 256, cache->kv_heads, a->batch), block, 0, s, p);

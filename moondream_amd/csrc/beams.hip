@@ -411,7 +411,7 @@ extern "C" md_status md_state_reorder(const md_state_part* parts, int32_t n_part
       const md_state_part& s = parts[done];
       const int width = width_of(s);
       const int64_t per = s.seg_bytes / width, words = words_of(s), mine = (words + 255) / 256;
-      if (groups + mine > 0x7fffffff) break;
+      if (groups + mine >= 1 << 24) break;  // (a launch has fewer than 2^32 threads)
       ps.p[ps.n++] = {(const char*)s.src, (char*)s.dst, s.src_slot_stride, s.dst_slot_stride, s.src_outer_stride, s.dst_outer_stride, s.src_seg_stride,
                       s.dst_seg_stride, (int32_t)per, s.segs, (int32_t)groups, width, (uint32_t)words};
       groups += mine;

@@ -373,7 +373,7 @@ extern "C" md_status md_kv8_append(const md_kv8_cache* cache, const void* k, int
   MD_CHECK_ARG((((uintptr_t)k | (uintptr_t)v) & 15) == 0 && (k_bs | k_ts | k_hs | v_bs | v_ts | v_hs) % 8 == 0);
   const int n_blocks = (int)(((int64_t)std::min(q_len, cache->ctx) + 2 * BLK - 2) / BLK);  // wherever in a block the first row falls
   const int64_t tasks = (int64_t)batch * n_blocks * 2 * cache->kv_heads, groups = (tasks + 3) / 4;
-  MD_CHECK_ARG(tasks <= 0x7fffffff);
+  MD_CHECK_ARG(groups <= MOST_GROUPS);
   const Rows rk{(const bf16_t*)k, k_bs, k_ts, k_hs}, rv{(const bf16_t*)v, v_bs, v_ts, v_hs};
   if (cache->head_dim == 64)
     hipLaunchKernelGGL(append_kernel<64>, dim3(groups), dim3(256), 0, (hipStream_t)stream, device_cache(cache), rk, rv, slot, row0, n_new, q_len, (uint32_t)n_blocks, (uint32_t)tasks);
@@ -388,7 +388,7 @@ extern "C" md_status md_kv8_read(const md_kv8_cache* cache, const int32_t* slot,
   MD_CHECK_ARG((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0);
   const int64_t chunks = (int64_t)rows * (cache->head_dim / 16), threads = chunks <= 128 ? 128 : 256, groups = (chunks + threads - 1) / threads;
   const int64_t all = groups * cache->kv_heads * 2 * batch;
-  MD_CHECK_ARG(all <= 0x7fffffff);
+  MD_CHECK_ARG(all <= MOST_GROUPS);
   if (cache->head_dim == 64)
     hipLaunchKernelGGL(read_kernel<64>, dim3(all), dim3(threads), 0, (hipStream_t)stream, device_cache(cache), slot, row0, kv_len, rows, (uint32_t)groups,
                        (bf16_t*)k_out, (bf16_t*)v_out);
@@ -414,7 +414,7 @@ extern "C" md_status md_kv8_evict(const md_kv8_cache* from, const md_kv8_cache* 
   }
   const int n_blocks = (a->keep + BLK - 1) / BLK;
   const int64_t heads2 = (int64_t)a->batch * from->kv_heads * 2, tasks = in_place ? heads2 : heads2 * n_blocks, groups = in_place ? tasks : (tasks + 3) / 4;
-  MD_CHECK_ARG(tasks <= 0x7fffffff);
+  MD_CHECK_ARG(groups <= (in_place ? MOST_GROUPS / 4 : MOST_GROUPS));
   hipStream_t s = (hipStream_t)stream;
 #define MD_SELECT(HELD, COPIES)                                                                                                                    \
   hipLaunchKernelGGL((select_kernel<HELD, COPIES>), dim3(from->kv_heads, a->batch), dim3(SEL), 0, s, a->weights, a->slot, a->kv_len, a->kept,      \

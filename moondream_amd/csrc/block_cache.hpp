@@ -38,6 +38,8 @@ __device__ __forceinline__ float kv8_magnitude(float x) {
   return a < __builtin_inff() ? a : 0.f;
 }
 
+constexpr int64_t MOST_GROUPS = (1 << 24) - 1;  // of 256 threads: a launch has fewer than 2^32
+
 inline bool kv8_cache_ok(const md_kv8_cache* c) {
   return c && c->k && c->v && c->k_exp && c->v_exp && (c->head_dim == 64 || c->head_dim == 128) && c->slots > 0 && c->kv_heads > 0 && c->ctx > 0 &&
          c->ctx % MD_KV8_BLOCK == 0 && c->slot_stride % 16 == 0 && c->slot_stride >= (int64_t)c->kv_heads * c->ctx * c->head_dim &&

@@ -428,6 +428,22 @@ def test_rows_that_stay_of_long_caches(ctx, keep):
             assert torch.equal(kept[b, h, : len(best)].cpu().long(), best) and bool((kept[b, h, len(best) :] == -1).all())
 
 
+def test_outputs_that_share_memory_are_refused():
+    c, _, _ = filled(torch.Generator().manual_seed(14), 2, 64, 2, 64)
+    q = torch.zeros(2, 3, 4, 64, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError):
+        c.attention(q, ints([5, 6]), out=torch.zeros(2, 1, 4, 64, dtype=BF16, device="cuda").expand(2, 3, 4, 64))
+
+
+def test_another_longest_in_every_step():
+    c, _, _ = filled(torch.Generator().manual_seed(15), 1, 2048, 1, 64)
+    q, n = torch.randn(1, 1, 1, 64, device="cuda").to(BF16), ints([9])
+    first = c.attention(q, n)
+    for longest in range(900, 2048):
+        out = c.attention(q, n, max_len=longest)
+    assert torch.equal(out, first) and len(c._workspaces) <= 1024
+
+
 @pytest.mark.parametrize("ctx", [96, 8192])
 def test_zeros_of_both_signs_are_equal_weights(ctx):
     c = BlockCache(1, ctx, 1, 64)

@@ -892,8 +892,9 @@ md_status md_kv8_read(const md_kv8_cache* cache, const int32_t* slot, const int3
  * weights (fp32 [slots][kv_heads][ctx], or NULL): weights[row] = decay * weights[row] + the sum over the sequence's queries and the
  * group's heads of the softmax weight that the row got, for the rows below kv_len; decay 0 does not read what was there.  With
  * weights a slot may appear once in a call.
- * Scores, softmax statistics, outputs and weights are held in fp32; a key's softmax weight enters the product with the values as fp16.  The order of
- * all sums follows from the counts of the call (not from the data): the same call gives the same bits.
+ * Scores, softmax statistics, outputs and weights are held in fp32; a key's softmax weight times its value block's scale enters the product with the values as
+ * fp16: with 11 bits down to 2^-21 of the query's largest such product, off by at most 2^-32 of that below.  The order of all sums follows from the counts of the
+ * call (not from the data): the same call gives the same bits.
  * q_len * (n_heads / kv_heads)^2 < 2^32, q_len * (n_heads / kv_heads) < 2^23, batch and kv_heads < 2^16. */
 typedef struct {
   const void* q;

@@ -6,13 +6,16 @@
 // converted once for all of them.  A wave holds NT tiles of 16 columns and walks over blocks of 32 keys, everything in registers:
 //   S^T [32 keys x 16 columns] = K Q^T       two tiles of v_mfma 16x16x32 bf16 per 32 coordinates; a lane's 16 bytes of a key row are its operand
 //                                            of two products (an e4m3 number is exact in bf16; which coordinates share a product is free)
-//   P = 2^(S * c + v_exp - m)                c = scale * log2(e) * 2^k_exp;  m the running maximum of the exponent
+//   P = 2^(S * c + v_exp - m)                c = scale * log2(e) * 2^k_exp;  m the running maximum of the exponent less 7
 //   O^T [head_dim x 16 columns] += V^T P     v_mfma 16x16x32 f16.  The accumulator layout of S^T is the operand layout of P (keys 4 q .. 4 q + 3 of
 //                                            both tiles in lane group q); V's operand is eight rows' bytes of one coordinate: a lane loads the
 //                                            same 4 (8) coordinates of its eight rows and transposes them with byte permutes
 // The value block's scale stands in the exponent (P holds p times 2^v_exp, V the bare codes), so blocks of any scales share one accumulator and
 // fp16's range is spent where the output is made: l = sum over blocks of 2^-v_exp * (the block's sum of P), and o = O / l.
-// m moves only when a column's exponent exceeds it by more than 8 (P <= 2^8): mostly one comparison instead of a reduction and a rescaling.
+// The largest P lies between 2^7 and 2^15, the top of fp16's range: a P keeps its 11 bits down to 2^-21 of the largest and something down to 2^-31.  (With the
+// largest at 1 the many small weights behind a first row that takes 0.99 of the sum were subnormal or lost: 32768 rows' outputs off by 13 to 28 %.)  fp16 because bf16 would keep 8 bits of
+// every weight, and a second product for the rest would double the work of the bound that there is.
+// m moves only when a column's exponent exceeds it by more than 15 (P <= 2^15): mostly one comparison instead of a reduction and a rescaling.
 //
 // Few columns (decode): the waves of a workgroup share a column tile and take its blocks in turn, several workgroups share the keys, and a second
 // kernel joins their (O, m, l).  Bound by the cache's bytes: 64 x 1003 rows of 32 heads of 64 (198 MB) in 38 us, 5.2 TB/s, the rate of a large copy.
@@ -32,7 +35,8 @@ namespace {
 constexpr int BLK = MD_KV8_BLOCK;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NO_MAX = -3.0e38f;   // running maximum before any key: 2^(-inf - NO_MAX) is 0, not NaN
-constexpr float SLACK = 8.f;
+constexpr float LIFT = 7.f;          // the largest P stands at 2^LIFT when the maximum moves,
+constexpr float SLACK = LIFT + 8.f;  // and at 2^SLACK, within fp16's 65504, before it does
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -212,7 +216,7 @@ __device__ __forceinline__ void softmax_block(f32x4 (&s)[NT][2], f16x8 (&pf)[NT]
   if (__any(over)) {
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) {
-      const float now = fmaxf(m[ct], over_q_max(top[ct])), f0 = __builtin_amdgcn_exp2f(m[ct] - now);
+      const float now = fmaxf(m[ct], over_q_max(top[ct]) - LIFT), f0 = __builtin_amdgcn_exp2f(m[ct] - now);
       m[ct] = now;
       l[ct] *= f0;
 #pragma unroll

@@ -6,8 +6,8 @@
 //   part_kernel    one workgroup per (beam, piece of the vocabulary): the piece in registers; each wave's largest logits, its maximum and its sum
 //                  of exponentials
 //   choose_kernel  one workgroup per input, one wave per beam: sums joined in 64 bits, the pieces' lists merged, totals; then the beams' lists merged
-// Four beams of 51200 logits: 6.2 + 5.2 us, two launches' latency; 64 rows of 51200 bf16 logits 11.4 + 5.8 us; 64 rows of 131075 fp32 ones 21 us (1.6 TB/s: the
-// vector instructions, some 1000 for a wave's 2048 logits, follow the loads, as all workgroups run at once) and 13.6 us for 16 beams.
+// Four beams of 51200 logits: 6.4 + 5.8 us, two launches' latency; 64 rows of 51200 bf16 logits 13.6 + 6.1 us; 64 rows of 131075 fp32 ones 27 us (1.2 TB/s: the
+// vector instructions, some 1700 for a wave's 2048 logits, 700 of them the sum's in 64 bits, follow the loads, as all workgroups run at once) and 13.9 us for 16 beams.
 // States move at 6.8 TB/s (16 x 4 beams, 1.6 GB in 235 us).
 #include "wave_ops.hpp"
 
@@ -35,9 +35,28 @@ __device__ __forceinline__ float value_of(uint64_t c) {
 }
 __device__ __forceinline__ uint32_t index_of(uint64_t c) { return ~(uint32_t)c; }
 
-// exp(x), x <= 0: the product's rounding is 2^-24 of its size, another one for each logit, so that sums of many are off by far less; terms whose
-// exponents are large, and off by more, are small
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
+// exp(x), x <= 0, in 64 bits: 2^n e^r with |r| <= log(2) / 2, of which the series up to r^11 leaves 2^-47 (r^12 / 12!).  In fp32 two beams whose sums differ by
+// less than some 2^-24 would be ranked by rounding.  (64 rows of 131075 logits: 21.7 us with fp32's exponential.)
+__device__ __forceinline__ double exp_of(double x) {
+  x = fmax(x, -750.);  // (e^-750 is 0)
+  const double n = rint(x * 1.4426950408889634), r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, x));  // (log(2) in two parts)
+  double p = 1. / 39916800;
+  p = fma(p, r, 1. / 3628800);
+  p = fma(p, r, 1. / 362880);
+  p = fma(p, r, 1. / 40320);
+  p = fma(p, r, 1. / 5040);
+  p = fma(p, r, 1. / 720);
+  p = fma(p, r, 1. / 120);
+  p = fma(p, r, 1. / 24);
+  p = fma(p, r, 1. / 6);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.);
+  p = fma(p, r, 1.);
+  return ldexp(p, (int)n);
+}
+
+// 16 bytes of a row at any multiple of its elements' size
+typedef u32x4 u32x4_anywhere __attribute__((aligned(2)));
 
 // a beam that has continuations of its own
 __device__ __forceinline__ bool goes_on(const float* scores, const int32_t* ended, int row) {
@@ -64,19 +83,19 @@ __global__ __launch_bounds__(256) void part_kernel(const T* __restrict__ logits,
   if (threadIdx.x < 8) lists[min(4 * beams + (int)threadIdx.x, 4 * MAXB - 1)] = 0;  // (the count runs over whole eights)
   __syncthreads();
   const T* x = logits + (int64_t)row * ld;
-  const int base = piece * PIECE - (int)(((uintptr_t)x & 15) / sizeof(T));  // (loads are aligned wherever the row begins: its first piece begins before it)
+  const int base = piece * PIECE;  // (who has which token follows from the token alone, not from where the row lies: equal rows have equal sums)
   float v[PER];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int at = base + (i * 256 + (int)threadIdx.x) * E;
-    if (at >= 0 && at + E <= vocab) {
-      const u32x4 w = *(const u32x4*)(x + at);
+    if (at + E <= vocab) {
+      const u32x4 w = *(const u32x4_anywhere*)(x + at);
       const T* e = (const T*)&w;
 #pragma unroll
       for (int j = 0; j < E; ++j) v[i * E + j] = logit<T>(e[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < E; ++j) v[i * E + j] = at + j >= 0 && at + j < vocab ? logit<T>(x[at + j]) : -INFINITY;
+      for (int j = 0; j < E; ++j) v[i * E + j] = at + j < vocab ? logit<T>(x[at + j]) : -INFINITY;
     }
   }
   const auto id_of = [&](int i) { return base + ((i / E) * 256 + (int)threadIdx.x) * E + i % E; };
@@ -94,12 +113,7 @@ __global__ __launch_bounds__(256) void part_kernel(const T* __restrict__ logits,
   double sum = 0.;
   if (m > -INFINITY) {
 #pragma unroll
-    for (int i = 0; i < PER; i += 4) {
-      float s4 = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s4 += exp_of(v[i + j] - m);
-      sum += (double)s4;
-    }
+    for (int i = 0; i < PER; ++i) sum += exp_of((double)v[i] - (double)m);
   }
   sum = wave_sum_f64(sum);
 
@@ -281,7 +295,7 @@ __global__ __launch_bounds__(64 * MAXB) void choose_kernel(int beams, int pieces
 int per_thread(int64_t rows, int vocab) { return rows * ((vocab + 256 * MANY - 1) / (256 * MANY)) >= 256 ? MANY : FEW; }
 size_t pieces_of(int64_t rows, int vocab) {
   const size_t piece = 256 * per_thread(rows, vocab);
-  return ((size_t)vocab + 7 + piece - 1) / piece;  // (up to 7 places before a row's first logit)
+  return ((size_t)vocab + piece - 1) / piece;
 }
 
 // ------------------------------------------------------------------------------------------------------------- states

@@ -1,0 +1,59 @@
+"""The choice among beams whose logits are alike, in rows of every alignment: sums of exponentials follow the tokens, not the addresses, and are in 64 bits."""
+import pytest
+import torch
+
+from moondream_amd.beams import select_beams
+
+import blocks_util as U
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.mark.parametrize("dtype, vocab", [(F32, 131075), (F32, 5001), (F32, 8191), (BF16, 8193), (BF16, 5001), (BF16, 51203), (F32, 4), (BF16, 9)])
+@pytest.mark.parametrize("batch, beams", [(1, 2), (2, 4), (7, 5), (3, 16)])
+def test_equal_rows_are_ties(dtype, vocab, batch, beams):
+    g = torch.Generator().manual_seed(vocab + beams)
+    for draw in range(4):
+        row = (torch.randn(batch, 1, vocab, generator=g) * 3).to(dtype)
+        if draw % 2:
+            row[:, 0, -1] = row.float().amax(-1)[:, 0].to(dtype) + 1  # the best token is the last one
+        logits = row.expand(batch, beams, vocab).reshape(batch * beams, vocab).cuda()
+        got = select_beams(logits, torch.full((batch, beams), -1.5, device="cuda"))
+        best = torch.sort(row[:, 0].double(), dim=-1, descending=True, stable=True)
+        for b in range(batch):  # rank by rank: all beams' best token, the lowest beam first
+            order = [(float(v), k, int(t)) for t, v in zip(best.indices[b, :beams], best.values[b, :beams]) for k in range(beams)]
+            order.sort(key=lambda c: (-c[0], c[1], c[2]))
+            assert got.parents[b].tolist() == [c[1] for c in order[:beams]] and got.tokens[b].tolist() == [c[2] for c in order[:beams]], draw
+            assert len({x for x, c in zip(got.scores[b].tolist(), order) if c[0] == order[0][0]}) == 1
+
+
+@pytest.mark.parametrize("dtype, vocab", [(F32, 131075), (F32, 5001), (BF16, 51203)])
+def test_sums_are_in_64_bits(dtype, vocab):
+    """Beams whose sums differ by some parts in 10^10: one rare token a little more likely in the lower beam, whose totals are the smaller ones for it."""
+    g = torch.Generator().manual_seed(vocab)
+    for draw in range(12):
+        row = (torch.randn(1, vocab, generator=g) * 3).to(dtype)
+        top = float(row.float().max())
+        logits = row.repeat(2, 1)
+        rare = int(torch.randint(0, vocab, (1,), generator=g))
+        logits[:, rare] = top - 20.0
+        logits[draw % 2, rare] = top - 19.0
+        scores = torch.zeros(1, 2)
+        want = U.beams(logits, scores[0], None, -1, -1, None)
+        got = select_beams(logits.cuda(), scores.cuda())
+        assert got.parents[0].tolist() == [w[1] for w in want] and got.tokens[0].tolist() == [w[0] for w in want]
+        assert want[0][1] == 1 - draw % 2
+        for x, w in zip(got.scores[0].tolist(), want):
+            assert abs(x - w[2]) <= abs(w[2]) * 2.0**-24 + 1e-12  # one rounding to fp32; sums in 64 bits
+
+
+def test_sums_of_far_apart_and_of_extreme_logits():
+    far = torch.tensor([[0.0, -80.0, -104.0, -500.0, -3e38], [3e38, 3e38, -3e38, 0.0, 1.0], [1e-40, -1e-40, 0.0, -0.0, 1e-45], [-3.4e38] * 5])
+    scores = torch.tensor([[-1.0, -2.0], [-3.0, -4.0]])
+    got = select_beams(far.cuda(), scores.cuda())
+    for b in range(2):
+        want = U.beams(far[2 * b : 2 * b + 2], scores[b], None, -1, -1, None)
+        assert got.tokens[b].tolist() == [w[0] for w in want] and got.parents[b].tolist() == [w[1] for w in want]
+        for x, w in zip(got.scores[b].tolist(), want):
+            assert abs(x - w[2]) <= abs(w[2]) * 2.0**-24 + 1e-12

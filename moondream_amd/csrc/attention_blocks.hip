@@ -765,13 +765,14 @@ __global__ __launch_bounds__(256, 4) void weights_kernel(Params p) {
 #pragma unroll
           for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (key0 + t * 16 + 4 * q + j >= lim) s[t][j] = -INFINITY;
+            for (int j = 0; j < 4; ++j)  // (a sum that is no number stays out of rows that its query does not see)
+              w[t][j] += key0 + t * 16 + 4 * q + j < lim ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j], ck[t], -ls)) : 0.f;
+        } else {
+#pragma unroll
+          for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[t][j] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j], ck[t], -ls));
         }
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) w[t][j] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j], ck[t], -ls));
       }
       __syncthreads();
     }

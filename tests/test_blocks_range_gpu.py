@@ -1,4 +1,6 @@
-"""Attention over long caches on the GPU: a first row that takes most of the weight, blocks that all matter, one sequence alone and in a batch."""
+"""Attention over long caches on the GPU: a first row that takes most of the weight, blocks that all matter, one sequence alone and in a batch, queries that are no numbers."""
+import math
+
 import pytest
 import torch
 
@@ -85,3 +87,23 @@ def test_a_sequence_alone_and_in_a_batch(dim, group, tokens):
         most, mass = max(most, float((x @ k.T).abs().max() * dim**-0.5)), max(mass, float((x.abs() @ k.abs().T).max() * dim**-0.5))
     for got in (w1, wb):
         assert bool(((got[0, heads - 1, :n].cpu().double() - want).abs() <= U.weights_tolerance(want, most, mass, dim, tokens * group)).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("tokens, group", [(4, 1), (9, 2), (100, 1), (300, 2)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_query_that_is_no_number_leaves_rows_alone_that_it_does_not_see(dim, tokens, group, bad):
+    g = torch.Generator().manual_seed(tokens)
+    n, heads = tokens + 45, 2
+    c = BlockCache(1, n, heads, dim)
+    x = torch.randn(1, n, heads, dim, generator=g).to(BF16).cuda()
+    c.append(x, x, ints([0]))
+    q = torch.randn(1, tokens, heads * group, dim, generator=g).to(BF16).cuda()
+    sick, well = q.clone(), q.clone()
+    at = tokens // 2
+    sick[0, at, 0, 5], well[0, at, 0] = bad, 0.0
+    w, clean = (torch.zeros(1, heads, c.ctx, device="cuda") for _ in range(2))
+    c.attention(sick, ints([n]), weights=w)
+    c.attention(well, ints([n]), weights=clean)
+    seen = n - tokens + at + 1
+    assert bool(torch.isnan(w[0, 0, :seen]).any()) and torch.equal(w[0, 0, seen:], clean[0, 0, seen:]) and torch.equal(w[0, 1], clean[0, 1])

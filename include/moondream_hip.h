@@ -886,8 +886,9 @@ md_status md_kv8_read(const md_kv8_cache* cache, const int32_t* slot, const int3
  * (query head h reads head h / (n_heads / kv_heads)).  q, o: bf16, element (b, t, h, d) at b * bs + t * ts + h * hs + d, 16-byte aligned,
  * strides % 8 == 0.  Query t of sequence b stands at row p = q_pos0[b] + t (q_pos0 NULL: the last q_rows[b] rows, kv_len[b] - q_rows[b] + t)
  * and sees the rows j <= p, with p < prefix_len all j < prefix_len, in every case j < kv_len[b] only; one that sees no row gives zeros.
- * Queries t >= q_rows[b] (NULL: q_len) are padding: their outputs stay as they are.  o may be q itself where no weights are wanted; else no element of
- * o is one of q.
+ * Queries t >= q_rows[b] (NULL: q_len) are padding: their outputs stay as they are.  o may be q itself, strides and all, where no weights are wanted; else no
+ * element of o is one of q, and no two elements of o are one.  Both are refused, and so is what is not told from them: strides of o of which one is
+ * less than the smaller ones span, and q and o of different strides in one range of memory.
  * max_len bounds kv_len (longer ones count as max_len; 0: ctx) and sizes the launch.
  * weights (fp32 [slots][kv_heads][ctx], or NULL): weights[row] = decay * weights[row] + the sum over the sequence's queries and the
  * group's heads of the softmax weight that the row got, for the rows below kv_len; decay 0 does not read what was there.  With

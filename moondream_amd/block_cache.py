@@ -146,7 +146,7 @@ class BlockCache:
         """Softmax attention of ``q`` [batch, tokens, heads, head_dim] (bf16) over the first ``kv_len[b]`` rows; returns the same shape.
 
         A sequence's queries are its last rows unless ``q_pos0`` says where the first one stands; each sees the rows up to its own, those in the first
-        ``prefix_len`` rows all of these.  ``out`` may be ``q`` itself where no weights are wanted.  ``q_rows``: how many of the queries count (the others' outputs stay as ``out`` has them; without
+        ``prefix_len`` rows all of these.  ``out`` may be ``q`` itself where no weights are wanted, and shares nothing with it otherwise.  ``q_rows``: how many of the queries count (the others' outputs stay as ``out`` has them; without
         ``out`` they are zeros).  ``max_len``: no sequence is longer (sizes the launch; longer ones are cut).  ``scale``: 1 / sqrt(head_dim).
         ``weights`` (fp32 [slots, kv_heads, ctx]) <- decay * weights + the softmax weight that every row got in this call."""
         qs = self._rows_of(q, "q")

@@ -25,6 +25,7 @@
 // Accumulators in the other half of the registers, which overlap, were slower (68 and 345 us: inline assembly that the compiler does not schedule), as were
 // scores of the next block made beside the softmax of this one (63 and 302 us: registers).
 #include "block_cache.hpp"
+#include "layout.hpp"
 #include "wave_ops.hpp"
 
 #include <algorithm>
@@ -858,6 +859,15 @@ bool args_ok(const md_kv8_cache* c, const md_kv8_attn_args* a) {
   return cols <= 0x7fffff && cols * (a->n_heads / c->kv_heads) < (1ll << 32) && a->batch <= 65535 && c->kv_heads <= 65535 && (a->slot || a->batch <= c->slots);
 }
 
+// o: elements of its own, and none of them one of q's but for q itself
+bool out_ok(const md_kv8_cache* c, const md_kv8_attn_args* a) {
+  const StridedRuns q{(uintptr_t)a->q, c->head_dim * 2, {a->batch, a->q_len, a->n_heads}, {a->q_bs * 2, a->q_ts * 2, a->q_hs * 2}};
+  const StridedRuns o{(uintptr_t)a->o, c->head_dim * 2, {a->batch, a->q_len, a->n_heads}, {a->o_bs * 2, a->o_ts * 2, a->o_hs * 2}};
+  if (!runs_apart_from_each_other(o)) return false;
+  if (a->o == (void*)a->q && runs_same_strides(q, o)) return !a->weights;  // (the weights are made from the queries again)
+  return !runs_meet(q, o);
+}
+
 }  // namespace
 
 extern "C" size_t md_kv8_attention_workspace_bytes(const md_kv8_cache* cache, const md_kv8_attn_args* args) {
@@ -867,7 +877,7 @@ extern "C" size_t md_kv8_attention_workspace_bytes(const md_kv8_cache* cache, co
 extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_attn_args* a, void* stream) {
   MD_CHECK_ARG(args_ok(cache, a) && a->q && a->o && a->kv_len && a->prefix_len >= 0);
   MD_CHECK_ARG((((uintptr_t)a->q | (uintptr_t)a->o) & 15) == 0 && (a->q_bs | a->q_ts | a->q_hs | a->o_bs | a->o_ts | a->o_hs) % 8 == 0);
-  MD_CHECK_ARG(!a->weights || a->o != (void*)a->q);  // (the weights are made from the queries again)
+  MD_CHECK_ARG(out_ok(cache, a));
   MD_CHECK_ARG(a->scale > -INFINITY && a->scale < INFINITY && (!a->weights || (a->decay >= 0.f && a->decay < INFINITY)));
   const Plan pl = plan_of(cache, a);
   if (pl.bytes && (!a->workspace || a->workspace_bytes < pl.bytes)) return MD_ERR_WORKSPACE;

@@ -57,7 +57,7 @@ struct Params {
   uint32_t per_group, all;  // 2^32 / group rounded up and 0; 0 and ~0 for a group of 1
   uint32_t q_sign;          // xor of two bf16 queries: a negative scale is taken as its magnitude and the queries negated, so that scores rise with products
   float scale_log2, decay;
-  float *scores;            // of few columns, with weights: [batch][kv_heads][cols][max_len to a whole block], in units of log2
+  float *scores;            // kept for the weights: [batch][kv_heads][cols][max_len to a whole block], in units of log2
   int score_rows, join_groups, batch, by_length, col_splits;
   float* wpart;             // of many columns shared out: [col_splits][batch][kv_heads][max_len to a whole block]
   float *part, *part_ml, *lse, *weights;  // part: [batch][kv_heads][cols][splits][head_dim], part_ml: ... [splits][2], lse: [batch][kv_heads][cols]
@@ -602,7 +602,7 @@ __device__ __forceinline__ float join_factor(const float* __restrict__ ml, int s
 }
 
 // After workgroups that shared keys.  The first join_groups workgroups of a head: one wave per column, its parts added in the splits' order.  The others (few
-// columns with weights): every row's softmax weights from the scores that the attention kernel left, 1024 rows each.
+// columns with kept scores): every row's softmax weights from the scores that the attention kernel left, 1024 rows each.
 template <int HD>
 __global__ __launch_bounds__(256) void join_kernel(Params p) {
   constexpr int N = HD / 64;
@@ -646,8 +646,8 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
     if (p.lse && lane == 0) p.lse[c0] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
     return;
   }
-  __shared__ float lse[32];
-  __shared__ int lims[32];
+  __shared__ float lse[24];  // (kept scores are those of up to 24 columns)
+  __shared__ int lims[24];
   const int first = (blockIdx.x - p.join_groups) * 1024;
   if (first >= sq.len) return;
   for (int col = wave; col < n_cols; col += 4) {
@@ -684,7 +684,7 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
     if (key + i < sq.len) out[i] = p.decay == 0.f ? w[i] : __builtin_fmaf(p.decay, out[i], w[i]);
 }
 
-// The weight that every row got from many columns.  A wave holds 32 keys as operands (64 would leave registers for two waves per SIMD, and exponentials and
+// The weight that every row got, from scores made again.  A wave holds 32 keys as operands (64 would leave registers for two waves per SIMD, and exponentials and
 // products of one wave follow each other: 201 us against 228 for 2 x 2048 queries over 6101 rows, 32 on 8 heads of 128); the columns that see them pass by, 64 at a time through LDS for the four waves.  Where that makes few workgroups the columns are shared out too (the first keys are
 // seen by all queries, the last by few: whole columns left 42 % of the CUs' time empty), and the shares added in their order afterwards.  The scores are the attention kernel's again (the same products in the same order), exp2(score - lse) is their softmax.
 template <int HD>
@@ -819,8 +819,11 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(Params p) {
 // Prompts: 32 columns a wave, 16 where more would stand empty (up to 64 columns) or where workgroups are few and short, so that one's latency counts, about
 // a microsecond a block (us, 32 / 16 columns: 767 queries of 32 heads of 64 17.0 / 13.0, 2048 of 32 on 8 heads of 128 76 / 64, but 512 queries of 64 on 8 heads
 // of 128 over 8192 rows 177 / 210).
+// Weights of few columns come from kept scores where these cost less than the keys and their products again: 8 bytes a key and column, there and back, which up to 3 columns for 16
+// coordinates is also a workspace of at most 3/8 of the cache's codes (us, kept / made again, 8 x 8 heads of 32768 keys: head size 64 with 4 columns 64 / 106, 12 95 / 104, 16 106 / 104,
+// 32 185 / 107; head size 128 with 4 columns 129 / 190, 16 170 / 195, 24 200 / 202, 32 241 / 206).
 struct Plan {
-  bool decode;
+  bool decode, kept;  // kept: few columns' scores stay in the workspace for the weights
   int nt, waves, col_groups, splits, cols, score_rows, col_splits;
   size_t part, ml, lse, scores, bytes;
 };
@@ -848,8 +851,9 @@ Plan plan_of(const md_kv8_cache* c, const md_kv8_attn_args* a) {
   const int64_t key_groups = (int64_t)((max_len + 127) / 128) * c->kv_heads * a->batch;
   pl.col_splits = (int)std::max<int64_t>(1, std::min<int64_t>({(3000 + key_groups - 1) / key_groups, (pl.cols + 255) / 256, 16}));
   pl.bytes = pl.scores;
-  if (a->weights && pl.decode) pl.bytes += (size_t)cols * pl.score_rows * 4;
-  if (a->weights && !pl.decode && pl.col_splits > 1) pl.bytes += (size_t)pl.col_splits * a->batch * c->kv_heads * pl.score_rows * 4;
+  pl.kept = a->weights && pl.decode && pl.cols * 16 <= 3 * c->head_dim;
+  if (pl.kept) pl.bytes += (size_t)cols * pl.score_rows * 4;
+  if (a->weights && !pl.kept && pl.col_splits > 1) pl.bytes += (size_t)pl.col_splits * a->batch * c->kv_heads * pl.score_rows * 4;
   return pl;
 }
 
@@ -913,7 +917,7 @@ extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_at
   p.part_ml = (float*)(ws + pl.ml);
   p.lse = a->weights ? (float*)(ws + pl.lse) : nullptr;
   p.weights = a->weights;
-  p.scores = a->weights && pl.decode ? (float*)(ws + pl.scores) : nullptr;
+  p.scores = pl.kept ? (float*)(ws + pl.scores) : nullptr;
   p.score_rows = pl.score_rows;
   p.wpart = (float*)(ws + pl.scores);
   p.col_splits = pl.col_splits;
@@ -922,7 +926,7 @@ extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_at
   p.join_groups = pl.splits > 1 ? (pl.cols + 3) / 4 : 0;
   const int64_t groups = (int64_t)pl.col_groups * pl.splits, all = groups * cache->kv_heads * a->batch;
   const int64_t key_groups = (int64_t)((p.max_len + 127) / 128) * cache->kv_heads * a->batch;
-  MD_CHECK_ARG((pl.decode || all <= MOST_GROUPS) && (pl.decode || !a->weights || key_groups <= MOST_GROUPS));
+  MD_CHECK_ARG((pl.decode || all <= MOST_GROUPS) && (pl.kept || !a->weights || key_groups <= MOST_GROUPS));
   const dim3 grid(groups, cache->kv_heads, a->batch), block(256);
   hipStream_t s = (hipStream_t)stream;
   if (pl.decode) {
@@ -960,7 +964,7 @@ extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_at
     else hipLaunchKernelGGL(join_kernel<128>, jg, block, 0, s, p);
     MD_TRY(md_launch_status());
   }
-  if (a->weights && !pl.decode) {
+  if (a->weights && !pl.kept) {
     const dim3 wg(key_groups, pl.col_splits);
     if (cache->head_dim == 64) hipLaunchKernelGGL(weights_kernel<64>, wg, block, 0, s, p);
     else hipLaunchKernelGGL(weights_kernel<128>, wg, block, 0, s, p);

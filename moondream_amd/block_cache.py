@@ -188,13 +188,15 @@ class BlockCache:
               into: Optional["BlockCache"] = None, into_weights: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """Of every sequence and head ``keep`` rows stay: the ``first`` ones, the ``recent`` last ones, and those of the largest ``weights`` (fp32
         [slots, kv_heads, ctx]; ties: the lower row).  They move together, in their order, to the rows 0 .. of the same slot -- of this
-        cache, or of ``into``, one of as many heads that shares no memory with it -- and their weights with them (in place, or to ``into_weights``
+        cache, or of ``into``, another of as many heads that shares no memory with it -- and their weights with them (in place, or to ``into_weights``
         [slots, kv_heads, ctx] of ``into``).  Returns the rows that stayed, int32 [batch, kv_heads, keep], -1 behind the last, and the new lengths."""
         to = self if into is None else into
         if to.device != self.device or (to.kv_heads, to.head_dim) != (self.kv_heads, self.head_dim):
             raise ValueError("into: a cache of as many heads of the same size on the same device")
         if into is None and into_weights is not None:
             raise ValueError("into_weights without into: in place the weights move within themselves")
+        if into is not None and all(a.data_ptr() == b.data_ptr() for a, b in ((self.k, to.k), (self.v, to.v), (self.k_exp, to.k_exp), (self.v_exp, to.v_exp))):
+            raise ValueError("into is this cache: leave it out, so that the weights move with their rows")
         if not (0 < keep <= to.ctx) or first < 0 or recent < 0 or first + recent > keep:
             raise ValueError(f"keep {keep}, first {first}, recent {recent}: wanted first + recent <= keep <= {to.ctx}")
         batch = kv_len.numel()

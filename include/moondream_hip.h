@@ -920,7 +920,8 @@ md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_attn_args* ar
 /* Eviction: of every sequence and head the rows [0, first), the last `recent` ones and those of the largest weights stay, `keep` in all
  * (all of them while kv_len[b] <= keep); ties: the lower row stays; a NaN weight is the least.  They move together to the rows 0 .. of the
  * same slot of `to`, in their order, every block with the scale that its rows need now.  `to` is the same cache (in place) or
- * one that shares no memory with it, of as many heads, the same head_dim and ctx >= keep.
+ * one that shares no memory with it, of as many heads, the same head_dim and ctx >= keep.  (Its slots may lie between those of the other at the same stride:
+ * another layer's in a slab.  Two strides in one range of memory are refused.)
  * weights: fp32 [slots][kv_heads][ctx] of `from`; weights_out: the same of `to` (in place: weights itself, so that they stay with their rows; NULL: not wanted,
  * `weights` stays as it is).
  * kept (int32 [batch][kv_heads][keep]): the rows that stayed, -1 behind the last;  len_out[b] = min(kv_len[b], keep), may be kv_len.

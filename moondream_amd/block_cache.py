@@ -196,7 +196,7 @@ class BlockCache:
         if into is None and into_weights is not None:
             raise ValueError("into_weights without into: in place the weights move within themselves")
         if into is not None and all(a.data_ptr() == b.data_ptr() for a, b in ((self.k, to.k), (self.v, to.v), (self.k_exp, to.k_exp), (self.v_exp, to.v_exp))):
-            raise ValueError("into is this cache: leave it out, so that the weights move with their rows")
+            raise ValueError("into lies in this cache's place: leave it out, so that the weights move with their rows")
         if not (0 < keep <= to.ctx) or first < 0 or recent < 0 or first + recent > keep:
             raise ValueError(f"keep {keep}, first {first}, recent {recent}: wanted first + recent <= keep <= {to.ctx}")
         batch = kv_len.numel()

@@ -6,6 +6,7 @@
 // (4.1 TB/s) and back in 34 us (4.3 TB/s), 4096 of 32749 rows of 8 x 8 heads of 128 gathered in 33 us (4.0 TB/s).  A single row per sequence is
 // latency: 64 sequences in 5.4 us.
 #include "block_cache.hpp"
+#include "layout.hpp"
 #include "wave_ops.hpp"
 
 #include <algorithm>
@@ -353,14 +354,17 @@ bool apart(const void* a, int64_t an, const void* b, int64_t bn) {
   return (uintptr_t)a + (uintptr_t)an <= (uintptr_t)b || (uintptr_t)b + (uintptr_t)bn <= (uintptr_t)a;
 }
 
-int64_t code_bytes(const md_kv8_cache* c) { return (c->slots - 1) * c->slot_stride + (int64_t)c->kv_heads * c->ctx * c->head_dim; }
-int64_t exp_bytes(const md_kv8_cache* c) { return (c->slots - 1) * c->exp_stride + (int64_t)c->kv_heads * (c->ctx / MD_KV8_BLOCK); }
+// keys, values and their scales, slot by slot (two layers' slots may lie between one another in a slab of all layers)
+StridedRuns slots_of(const md_kv8_cache* c, int which) {
+  const void* at[4] = {c->k, c->v, c->k_exp, c->v_exp};
+  const int64_t rows = which < 2 ? (int64_t)c->ctx * c->head_dim : c->ctx / MD_KV8_BLOCK;
+  return {(uintptr_t)at[which], c->kv_heads * rows, {c->slots, 1, 1}, {which < 2 ? c->slot_stride : c->exp_stride, 0, 0}};
+}
 
 bool caches_apart(const md_kv8_cache* a, const md_kv8_cache* b) {
-  const void *pa[4] = {a->k, a->v, a->k_exp, a->v_exp}, *pb[4] = {b->k, b->v, b->k_exp, b->v_exp};
   for (int i = 0; i < 4; ++i)
     for (int j = 0; j < 4; ++j)
-      if (!apart(pa[i], i < 2 ? code_bytes(a) : exp_bytes(a), pb[j], j < 2 ? code_bytes(b) : exp_bytes(b))) return false;
+      if (runs_meet(slots_of(a, i), slots_of(b, j))) return false;
   return true;
 }
 

@@ -4,7 +4,7 @@ import torch
 
 from moondream_amd.block_cache import BlockCache
 
-from test_blocks_gpu import filled, ints
+from test_blocks_gpu import filled, ints, random_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -20,3 +20,44 @@ def test_a_cache_into_itself_is_refused(of):
         with pytest.raises(ValueError):
             c.evict(w, ints([96, 90]), 40, into=into, into_weights=into_weights)
     assert torch.equal(before[0], c.k) and torch.equal(before[1], w)
+
+
+@pytest.mark.parametrize("keep", [40, 64])
+def test_from_one_layer_s_slots_into_another_s_between_them(keep):
+    """Slabs [slots, layers, ...]: the layers' slots lie between one another and share no byte."""
+    g = torch.Generator().manual_seed(3)
+    slots, heads, ctx, dim = 3, 2, 96, 64
+    whole = [torch.zeros(slots, 3, heads, ctx, dim, dtype=torch.uint8, device="cuda") for _ in range(2)] + [torch.full((slots, 3, heads, ctx // 32), 87, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    layers = [BlockCache.of(*(t[:, i] for t in whole)) for i in range(3)]
+    x, y = (random_rows(g, slots, ctx, heads, dim).cuda() for _ in range(2))
+    alone, into = BlockCache(slots, ctx, heads, dim), BlockCache(slots, ctx, heads, dim)
+    for c in (layers[1], alone):
+        c.append(x, y, ints([0] * slots))
+    w = torch.rand(slots, heads, ctx, generator=g).cuda()
+    w1, w2 = torch.zeros_like(w), torch.zeros_like(w)
+    lens = ints([96, 50, 30])
+    before = [t[:, 1].clone() for t in whole]
+    for to, out in ((layers[2], w1), (layers[0], w1)):
+        kept, n = layers[1].evict(w, lens, keep, recent=8, into=to, into_weights=out)
+        kept2, n2 = alone.evict(w, lens, keep, recent=8, into=into, into_weights=w2)
+        assert torch.equal(kept, kept2) and torch.equal(n, n2) and torch.equal(w1, w2)
+        for a, b in zip(to.read(None, ctx, kv_len=n), into.read(None, ctx, kv_len=n)):
+            assert torch.equal(a, b)
+    assert all(torch.equal(t[:, 1], b) for t, b in zip(whole, before))
+
+
+def test_caches_that_share_some_slots_are_refused():
+    from moondream_amd._lib import MoondreamHipError
+
+    c, _, _ = filled(torch.Generator().manual_seed(2), 4, 64, 2, 64)
+    first, last = (BlockCache.of(*(t[s] for t in (c.k, c.v, c.k_exp, c.v_exp))) for s in (slice(0, 3), slice(1, 4)))
+    w = torch.rand(3, 2, 64, device="cuda")
+    even = BlockCache.of(*(t[::2] for t in (c.k, c.v, c.k_exp, c.v_exp)))
+    odd = BlockCache.of(*(t[1::2] for t in (c.k, c.v, c.k_exp, c.v_exp)))
+    before = c.k.clone()
+    for a, b in ((first, last), (last, first), (first, even)):
+        with pytest.raises((ValueError, MoondreamHipError)):
+            a.evict(w[: a.slots].contiguous(), ints([64] * 2), 8, into=b)
+    assert torch.equal(c.k, before)
+    even.evict(w[:2].contiguous(), ints([64] * 2), 8, into=odd)
+    assert torch.equal(c.k[::2], before[::2])

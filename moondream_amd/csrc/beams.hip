@@ -9,6 +9,7 @@
 // Four beams of 51200 logits: 6.4 + 5.8 us, two launches' latency; 64 rows of 51200 bf16 logits 13.6 + 6.1 us; 64 rows of 131075 fp32 ones 27 us (1.2 TB/s: the
 // vector instructions, some 1700 for a wave's 2048 logits, 700 of them the sum's in 64 bits, follow the loads, as all workgroups run at once) and 13.9 us for 16 beams.
 // States move at 6.8 TB/s (16 x 4 beams, 1.6 GB in 235 us).
+#include "layout.hpp"
 #include "wave_ops.hpp"
 
 #include <algorithm>
@@ -351,11 +352,6 @@ __global__ __launch_bounds__(256) void reorder_kernel(Parts parts, const int32_t
   else move_words<uint8_t, B>(p, first, parents + slot0, beams, slot0);
 }
 
-int64_t extent(const md_state_part& s, bool src, int64_t slots) {
-  const int64_t a = src ? s.src_slot_stride : s.dst_slot_stride, b = src ? s.src_outer_stride : s.dst_outer_stride, c = src ? s.src_seg_stride : s.dst_seg_stride;
-  return (slots - 1) * a + (s.outer - 1) * b + (s.segs - 1) * c + s.seg_bytes;
-}
-
 // bytes that a thread moves at once, and how many such words a slot has
 int width_of(const md_state_part& s) {
   const uint64_t all = (uint64_t)s.src | (uint64_t)s.dst | (uint64_t)s.src_slot_stride | (uint64_t)s.dst_slot_stride | (uint64_t)s.src_outer_stride |
@@ -372,11 +368,11 @@ bool part_ok(const md_state_part& s, int64_t slots) {
   const int64_t strides[6] = {s.src_slot_stride, s.dst_slot_stride, s.src_outer_stride, s.dst_outer_stride, s.src_seg_stride, s.dst_seg_stride};
   for (int64_t x : strides)
     if (x < 0) return false;
-  if ((s.dst_slot_stride < s.seg_bytes && slots > 1) || (s.dst_outer_stride < s.seg_bytes && s.outer > 1) || (s.dst_seg_stride < s.seg_bytes && s.segs > 1))
-    return false;  // (two runs would be written to one place)
+  const StridedRuns src{(uintptr_t)s.src, s.seg_bytes, {slots, s.outer, s.segs}, {s.src_slot_stride, s.src_outer_stride, s.src_seg_stride}};
+  const StridedRuns dst{(uintptr_t)s.dst, s.seg_bytes, {slots, s.outer, s.segs}, {s.dst_slot_stride, s.dst_outer_stride, s.dst_seg_stride}};
+  if (!runs_apart_from_each_other(dst)) return false;  // (two runs would be written to one place)
   if (s.src == s.dst) return s.src_slot_stride == s.dst_slot_stride && s.src_outer_stride == s.dst_outer_stride && s.src_seg_stride == s.dst_seg_stride;
-  const uintptr_t a = (uintptr_t)s.src, b = (uintptr_t)s.dst;
-  return a + (uintptr_t)extent(s, true, slots) <= b || b + (uintptr_t)extent(s, false, slots) <= a;
+  return !runs_meet(src, dst);
 }
 
 }  // namespace

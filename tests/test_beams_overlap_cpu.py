@@ -1,0 +1,15 @@
+"""States whose runs would be written over one another: refused.  No GPU, nothing is launched."""
+import ctypes as C
+
+import pytest
+
+from moondream_amd import _lib
+
+from test_blocks_cpu import AT, part
+
+
+@pytest.mark.parametrize("bad", [dict(src_slot_stride=64, dst_slot_stride=64, src_seg_stride=64, dst_seg_stride=64), dict(dst_slot_stride=128), dict(outer=2, src_outer_stride=1024, dst_outer_stride=1024),
+                                 dict(dst=AT, src_slot_stride=192, dst_slot_stride=192), dict(dst=AT + 256), dict(dst=AT + 32, src_seg_stride=128, dst_seg_stride=128, src_slot_stride=512, dst_slot_stride=512),
+                                 dict(dst=AT + 64, src_seg_stride=128, dst_seg_stride=192, src_slot_stride=512, dst_slot_stride=768)], ids=str)
+def test_reordering_refuses_runs_that_meet(bad):
+    assert _lib.load().md_state_reorder(C.byref(part(**bad)), 1, AT, 2, 4, None) == 1

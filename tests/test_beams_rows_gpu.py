@@ -57,3 +57,21 @@ def test_sums_of_far_apart_and_of_extreme_logits():
         assert got.tokens[b].tolist() == [w[0] for w in want] and got.parents[b].tolist() == [w[1] for w in want]
         for x, w in zip(got.scores[b].tolist(), want):
             assert abs(x - w[2]) <= abs(w[2]) * 2.0**-24 + 1e-12
+
+
+@pytest.mark.parametrize("beams", [2, 5])
+def test_states_between_one_another(beams):
+    """From one layer's part of a slab [slots, layers, ...] into another's, and from some rows of an answer to others: ranges that overlap, no byte in common."""
+    from moondream_amd.beams import reorder_states
+
+    g = torch.Generator().manual_seed(beams)
+    n = 3 * beams
+    slab = torch.randn(n, 3, 4, 50, 16, generator=g).cuda()
+    parents = torch.randint(0, beams, (3, beams), generator=g)
+    slots = (parents + torch.arange(3)[:, None] * beams).view(-1).cuda()
+    want = slab.clone()
+    want[:, 2] = slab[slots, 1]
+    want[:, 0, :, 30:41] = slab[slots, 0, :, 3:14]
+    reorder_states([slab[:, 1]], parents.to(torch.int32).cuda(), into=[slab[:, 2]])
+    reorder_states([slab[:, 0, :, 3:14]], parents.to(torch.int32).cuda(), into=[slab[:, 0, :, 30:41]])
+    assert torch.equal(slab, want)

@@ -872,10 +872,16 @@ typedef struct {
 /* Rows row0[b] .. row0[b] + n_new[b] - 1 of every sequence (n_new NULL: q_len) from bf16 keys and values, element (b, t, h, d) at
  * b * bs + t * ts + h * hs + d, 16-byte aligned, strides % 8 == 0.  Rows past ctx are dropped.  A block that began before row0 keeps at
  * least its scale; where the new rows need a larger one its older rows are rounded to that.  The new rows are the sequence's last: rows behind
- * them in their last block count as gone (their codes stay, under the block's new scale).  All other blocks stay as they are. */
+ * them in their last block count as gone (their codes stay, under the block's new scale).  All other blocks stay as they are.  A row0[b] outside
+ * [0, ctx) writes nothing. */
 md_status md_kv8_append(const md_kv8_cache* cache, const void* k, int64_t k_bs, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_bs,
                         int64_t v_ts, int64_t v_hs, const int32_t* slot, const int32_t* row0, const int32_t* n_new, int32_t batch,
                         int32_t q_len, void* stream);
+/* The same, and the new rows begin without weight: weights[slot][h][row] = 0 (fp32 [slots][kv_heads][ctx], what md_kv8_attention adds to; NULL: none).  Where rows
+ * were evicted, or a slot had another sequence before, the weights of rows that are no more stand there. */
+md_status md_kv8_append_weighted(const md_kv8_cache* cache, const void* k, int64_t k_bs, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_bs,
+                                 int64_t v_ts, int64_t v_hs, const int32_t* slot, const int32_t* row0, const int32_t* n_new, float* weights,
+                                 int32_t batch, int32_t q_len, void* stream);
 
 /* Rows row0[b] .. row0[b] + rows - 1 as bf16 (exactly what the codes stand for): k_out, v_out contiguous [batch][kv_heads][rows][head_dim],
  * 16-byte aligned.  Rows outside [0, min(kv_len[b], ctx)) (kv_len NULL: ctx) read as zeros; row0 NULL: 0. */
@@ -924,6 +930,7 @@ md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_attn_args* ar
  * another layer's in a slab.  Two strides in one range of memory are refused.)
  * weights: fp32 [slots][kv_heads][ctx] of `from`; weights_out: the same of `to` (in place: weights itself, so that they stay with their rows; NULL: not wanted,
  * `weights` stays as it is).
+ * Codes, scales and weights behind the last row that stayed are left as they are.
  * kept (int32 [batch][kv_heads][keep]): the rows that stayed, -1 behind the last;  len_out[b] = min(kv_len[b], keep), may be kv_len.
  * A slot may appear once in a call; one outside either cache is an absent sequence.  first + recent <= keep. */
 typedef struct {

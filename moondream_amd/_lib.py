@@ -319,6 +319,8 @@ SIGNATURES = {
     "md_lm_set_kernels": (None, [c_int32]),
     "md_kv8_append": (C.c_int, [P(MdKv8Cache), c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p,
                                 c_void_p, c_int32, c_int32, c_void_p]),
+    "md_kv8_append_weighted": (C.c_int, [P(MdKv8Cache), c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                         c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
     "md_kv8_read": (C.c_int, [P(MdKv8Cache), c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
     "md_kv8_attention_workspace_bytes": (c_size_t, [P(MdKv8Cache), P(MdKv8AttnArgs)]),
     "md_kv8_attention": (C.c_int, [P(MdKv8Cache), P(MdKv8AttnArgs), c_void_p]),

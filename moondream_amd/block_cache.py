@@ -3,7 +3,7 @@
 ``BlockCache`` is one layer's cache of any number of sequences (slots).  It needs no calibration: a block's scale follows from the rows
 that are in it (include/moondream_hip.h, md_kv8_cache).  A decode step of a layer is::
 
-    cache.append(k, v, row0=length)                     # the new tokens' rows
+    cache.append(k, v, row0=length, weights=w)          # the new tokens' rows, without weight so far
     o = cache.attention(q, length + 1, weights=w)       # ... and what they see; w: the weight that every cached row got so far
     kept, length = cache.evict(w, length + 1, keep=4096, recent=256)   # now and then: the rows of least weight leave
 
@@ -106,10 +106,12 @@ class BlockCache:
             raise ValueError(f"{name}: rows of head_dim have to be contiguous and 16-byte aligned (strides {s})")
         return s
 
-    def append(self, k: torch.Tensor, v: torch.Tensor, row0: torch.Tensor, new: Optional[torch.Tensor] = None, slot: Optional[torch.Tensor] = None) -> None:
+    def append(self, k: torch.Tensor, v: torch.Tensor, row0: torch.Tensor, new: Optional[torch.Tensor] = None, slot: Optional[torch.Tensor] = None,
+               weights: Optional[torch.Tensor] = None) -> None:
         """Rows row0[b] .. of every sequence from bf16 ``k``, ``v`` [batch, tokens, kv_heads, head_dim] (views of a projection's rows will do; keys
         rotated already); ``new``: how many of the tokens count, per sequence.  Rows past ``ctx`` are dropped.  The new rows are the sequence's last (what lay behind
-        them in their last block is gone).  A slot at most once."""
+        them in their last block is gone).  ``weights`` (fp32 [slots, kv_heads, ctx], what ``attention`` adds to): the new rows' become 0; without it they keep what an evicted
+        row, or the slot's sequence before, left there.  A slot at most once."""
         ks, vs = self._rows_of(k, "k"), self._rows_of(v, "v")
         shape = k.shape
         batch, tokens, heads, _ = shape
@@ -119,9 +121,9 @@ class BlockCache:
         if tokens == 0:
             return
         of = (batch,)
-        _launch(self._index, "md_kv8_append", self._lib.md_kv8_append, self._ref, k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
+        _launch(self._index, "md_kv8_append", self._lib.md_kv8_append_weighted, self._ref, k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
                 None if slot is None else _need(slot, "slot", _I32, self._index, of), _need(row0, "row0", _I32, self._index, of),
-                None if new is None else _need(new, "new", _I32, self._index, of), batch, tokens)
+                None if new is None else _need(new, "new", _I32, self._index, of), self._weights(weights, "weights"), batch, tokens)
 
     def read(self, row0: Optional[torch.Tensor], rows: int, kv_len: Optional[torch.Tensor] = None, slot: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """Rows row0[b] .. row0[b] + rows - 1 (None: from 0) as bf16 [batch, kv_heads, rows, head_dim] keys and values, exactly what the codes stand
@@ -189,7 +191,7 @@ class BlockCache:
         """Of every sequence and head ``keep`` rows stay: the ``first`` ones, the ``recent`` last ones, and those of the largest ``weights`` (fp32
         [slots, kv_heads, ctx]; ties: the lower row).  They move together, in their order, to the rows 0 .. of the same slot -- of this
         cache, or of ``into``, another of as many heads that shares no memory with it -- and their weights with them (in place, or to ``into_weights``
-        [slots, kv_heads, ctx] of ``into``).  Returns the rows that stayed, int32 [batch, kv_heads, keep], -1 behind the last, and the new lengths."""
+        [slots, kv_heads, ctx] of ``into``); what lies behind the last that stayed is left as it is (``append`` clears the weights of rows that come there).  Returns the rows that stayed, int32 [batch, kv_heads, keep], -1 behind the last, and the new lengths."""
         to = self if into is None else into
         if to.device != self.device or (to.kv_heads, to.head_dim) != (self.kv_heads, self.head_dim):
             raise ValueError("into: a cache of as many heads of the same size on the same device")

@@ -33,7 +33,8 @@ struct Rows {
 // One wave per (sequence, block that the new rows touch, K or V, head); heads next to one another, as a token's heads are in memory.
 template <int HD>
 __global__ __launch_bounds__(256) void append_kernel(Cache c, Rows k, Rows v, const int32_t* __restrict__ slot, const int32_t* __restrict__ row0,
-                                                     const int32_t* __restrict__ n_new, int q_len, uint32_t n_blocks, uint32_t n_tasks) {
+                                                     const int32_t* __restrict__ n_new, float* __restrict__ weights, int q_len, uint32_t n_blocks,
+                                                     uint32_t n_tasks) {
   constexpr int CPR = HD / 8, N = BLK * CPR / 64;  // chunks of 8 coordinates: per row, per lane
   const int lane = threadIdx.x & 63;
   uint32_t task = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -98,6 +99,8 @@ __global__ __launch_bounds__(256) void append_kernel(Cache c, Rows k, Rows v, co
     *(u32x2*)(codes + ch * 8) = w;
   }
   if (lane == 0) *ep = (uint8_t)(e + 127);
+  if (weights && which == 0 && lane < BLK && base + lane >= r0 && base + lane < end)  // (what an evicted row or the slot's last sequence left there)
+    weights[((int64_t)sl * c.heads + h) * c.ctx + base + lane] = 0.f;
 }
 
 // 16 coordinates per thread: 16 bytes in, 32 out.  A workgroup belongs to one head's keys or values of one sequence, so that all but the row is the same
@@ -373,6 +376,12 @@ bool caches_apart(const md_kv8_cache* a, const md_kv8_cache* b) {
 extern "C" md_status md_kv8_append(const md_kv8_cache* cache, const void* k, int64_t k_bs, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_bs,
                                    int64_t v_ts, int64_t v_hs, const int32_t* slot, const int32_t* row0, const int32_t* n_new, int32_t batch,
                                    int32_t q_len, void* stream) {
+  return md_kv8_append_weighted(cache, k, k_bs, k_ts, k_hs, v, v_bs, v_ts, v_hs, slot, row0, n_new, nullptr, batch, q_len, stream);
+}
+
+extern "C" md_status md_kv8_append_weighted(const md_kv8_cache* cache, const void* k, int64_t k_bs, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_bs,
+                                            int64_t v_ts, int64_t v_hs, const int32_t* slot, const int32_t* row0, const int32_t* n_new, float* weights,
+                                            int32_t batch, int32_t q_len, void* stream) {
   MD_CHECK_ARG(kv8_cache_ok(cache) && k && v && row0 && batch > 0 && q_len > 0 && (slot || batch <= cache->slots));
   MD_CHECK_ARG((((uintptr_t)k | (uintptr_t)v) & 15) == 0 && (k_bs | k_ts | k_hs | v_bs | v_ts | v_hs) % 8 == 0);
   const int n_blocks = (int)(((int64_t)std::min(q_len, cache->ctx) + 2 * BLK - 2) / BLK);  // wherever in a block the first row falls
@@ -380,9 +389,9 @@ extern "C" md_status md_kv8_append(const md_kv8_cache* cache, const void* k, int
   MD_CHECK_ARG(groups <= MOST_GROUPS);
   const Rows rk{(const bf16_t*)k, k_bs, k_ts, k_hs}, rv{(const bf16_t*)v, v_bs, v_ts, v_hs};
   if (cache->head_dim == 64)
-    hipLaunchKernelGGL(append_kernel<64>, dim3(groups), dim3(256), 0, (hipStream_t)stream, device_cache(cache), rk, rv, slot, row0, n_new, q_len, (uint32_t)n_blocks, (uint32_t)tasks);
+    hipLaunchKernelGGL(append_kernel<64>, dim3(groups), dim3(256), 0, (hipStream_t)stream, device_cache(cache), rk, rv, slot, row0, n_new, weights, q_len, (uint32_t)n_blocks, (uint32_t)tasks);
   else
-    hipLaunchKernelGGL(append_kernel<128>, dim3(groups), dim3(256), 0, (hipStream_t)stream, device_cache(cache), rk, rv, slot, row0, n_new, q_len, (uint32_t)n_blocks, (uint32_t)tasks);
+    hipLaunchKernelGGL(append_kernel<128>, dim3(groups), dim3(256), 0, (hipStream_t)stream, device_cache(cache), rk, rv, slot, row0, n_new, weights, q_len, (uint32_t)n_blocks, (uint32_t)tasks);
   return md_launch_status();
 }
 

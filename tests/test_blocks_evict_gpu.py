@@ -61,3 +61,55 @@ def test_caches_that_share_some_slots_are_refused():
     assert torch.equal(c.k, before)
     even.evict(w[:2].contiguous(), ints([64] * 2), 8, into=odd)
     assert torch.equal(c.k[::2], before[::2])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_rows_that_come_after_an_eviction_begin_without_weight(dim, tokens):
+    """Steps as a program runs them: rows in, attention, an eviction in place, rows in where evicted ones were; then a new sequence in a used slot."""
+    import blocks_util as U
+
+    g = torch.Generator().manual_seed(dim + tokens)
+    heads, ctx = 2, 160
+    c, w = BlockCache(3, ctx, heads, dim), torch.zeros(3, heads, ctx, device="cuda")
+    slot, length = ints([2, 0]), ints([0, 0])
+
+    def step(length):
+        x, y, q = (random_rows(g, 2, tokens, heads, dim, spread=0.5).cuda() for _ in range(3))
+        c.append(x, y, length, slot=slot, weights=w)
+        length = length + tokens
+        c.attention(q, length, slot=slot, weights=w)
+        return q.cpu(), length
+
+    for _ in range(100 // tokens):
+        _, length = step(length)
+    had = w.cpu()
+    kept, length = c.evict(w, length, 20, recent=4, slot=slot)
+    assert length.tolist() == [20, 20] and bool((w[2, :, 20 : 20 + tokens] != 0).any())
+    for fresh in (False, True):
+        if fresh:
+            length = ints([0, 0])
+        before = torch.zeros(3, heads, ctx, dtype=torch.float64) if fresh else w.cpu().double()
+        start = int(length[0])
+        q, length = step(length)
+        k, v = (U.held(t.cpu(), e.cpu()) for t, e in ((c.k, c.k_exp), (c.v, c.v_exp)))
+        for b, s in enumerate((2, 0)):
+            n = start + tokens
+            _, want, _, most, mass = U.attention(q[b], k[s], v[s], n, start, 0, dim**-0.5)
+            want[:, :start] += before[s, :, :start]
+            near = (w[s, :, :n].cpu().double() - want[:, :n]).abs()
+            assert bool((near <= U.weights_tolerance(want[:, :n], most, mass, dim, tokens) + want[:, :n] * 2.0**-23).all())
+    assert not bool(w[1].any()) and bool((had[0] != 0).any())
+
+
+def test_the_weights_of_rows_that_are_not_new_stay():
+    c, w = BlockCache(4, 96, 3, 64), torch.ones(4, 3, 96, device="cuda")
+    x = torch.ones(5, 40, 3, 64, dtype=torch.bfloat16, device="cuda")
+    c.append(x, x, ints([10, 90, 31, -1, 0]), new=ints([40, 9, 0, 5, 33]), slot=ints([3, 0, 1, 1, 4]), weights=w)
+    want = torch.ones(4, 3, 96)
+    want[3, :, 10:50] = 0
+    want[0, :, 90:] = 0
+    assert torch.equal(w.cpu(), want)
+    for bad in (w[:3], w.double(), w[:, :, :95], w.cpu()):
+        with pytest.raises(ValueError):
+            c.append(x, x, ints([0] * 5), slot=ints([3, 0, 1, 1, 4]), weights=bad)

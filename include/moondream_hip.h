@@ -957,7 +957,8 @@ md_status md_kv8_evict(const md_kv8_cache* from, const md_kv8_cache* to, const m
  *   tokens, parents [batch][beams]: the token, and the beam (of the same input) that it goes on from
  *   scores_out: its total;  ended_out: its beam had ended or the token is end_id.  May be scores / ended.
  * Where fewer continuations are left: token end_id, parent the place itself, score -inf, ended.
- * ended NULL: none has; end_id -1: no token ends a beam (then ended is NULL).  ended_out may be NULL.  2 <= beams <= MD_MAX_BEAMS. */
+ * ended NULL: none has; end_id -1: no token ends a beam (then ended is NULL).  ended_out may be NULL.  2 <= beams <= MD_MAX_BEAMS,
+ * vocab < 2^31 - 8192. */
 #define MD_MAX_BEAMS 16
 typedef struct {
   const void* logits;

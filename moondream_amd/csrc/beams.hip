@@ -22,6 +22,7 @@ constexpr int MANY = 32, FEW = 8;
 constexpr int MAXB = MD_MAX_BEAMS;
 constexpr int LISTED = 7680;  // candidates of an input that choose_kernel has in LDS (30 pieces of 16 beams, 64 of up to 10)
 constexpr int ROOM = 128;    // logits of a wave that are put in order together
+constexpr int MOST_VOCAB = 0x7fffffff - 256 * MANY;  // (the places of the last piece are counted in 32 bits)
 constexpr float F32_MOST = 3.4028234663852886e38f;
 
 // (value, index) as one number: the larger value first, of equal ones the lower index.  0 stands for nothing.
@@ -300,7 +301,7 @@ size_t pieces_of(int64_t rows, int vocab) {
 }
 
 // ------------------------------------------------------------------------------------------------------------- states
-constexpr int MAX_PARTS = 32;  // of a launch (80 bytes each in its arguments)
+constexpr int MAX_PARTS = 32;  // of a launch (88 bytes each in its arguments)
 
 struct Part {
   const char* src;
@@ -378,12 +379,12 @@ bool part_ok(const md_state_part& s, int64_t slots) {
 }  // namespace
 
 extern "C" size_t md_beam_workspace_bytes(int32_t batch, int32_t beams, int32_t vocab) {
-  if (batch <= 0 || beams < 2 || beams > MAXB || vocab <= 0) return 0;
+  if (batch <= 0 || beams < 2 || beams > MAXB || vocab <= 0 || vocab > MOST_VOCAB) return 0;
   return (size_t)batch * beams * pieces_of((int64_t)batch * beams, vocab) * (beams * sizeof(uint64_t) + 2 * sizeof(double));
 }
 
 extern "C" md_status md_beam_select(const md_beam_args* a, void* stream) {
-  MD_CHECK_ARG(a && a->logits && a->scores && a->tokens && a->parents && a->scores_out && a->batch > 0 && a->vocab > 0 && a->ld >= a->vocab);
+  MD_CHECK_ARG(a && a->logits && a->scores && a->tokens && a->parents && a->scores_out && a->batch > 0 && a->vocab > 0 && a->vocab <= MOST_VOCAB && a->ld >= a->vocab);
   MD_CHECK_ARG(a->beams >= 2 && a->beams <= MAXB && (a->dtype == MD_DTYPE_BF16 || a->dtype == MD_DTYPE_F32) && (int64_t)a->batch * a->beams <= 65535);
   MD_CHECK_ARG(a->end_id < a->vocab && (a->end_id >= 0 || !a->ended) && ((uintptr_t)a->logits & (a->dtype == MD_DTYPE_F32 ? 3 : 1)) == 0);
   const int rows = a->batch * a->beams, pieces = (int)pieces_of(rows, a->vocab);

@@ -980,7 +980,8 @@ md_status md_beam_select(const md_beam_args* args, void* stream);
 /* States behind their parents: slot b * beams + k of dst = slot b * beams + parents[b][k] of src, for each of n_parts pieces of state.  A piece
  * is `outer` x `segs` runs of seg_bytes bytes in every slot, run (i, j) at slot * slot_stride + i * outer_stride + j * seg_stride
  * (bytes).  dst == src with equal strides: in place (only what changes its slot is read and written); else the two share no memory (runs between the other's at
- * the same strides are apart; different strides in one range of memory are refused).  Of dst's strides each is at least what the smaller ones span.  A parent
+ * the same strides are apart; different strides in one range of memory are refused).  Of dst's strides each is at least what the smaller ones span.  What one
+ * piece writes no other piece reads or writes (refused where the two begin at one address).  A parent
  * outside [0, beams): the slot itself.  1 <= beams <= MD_MAX_BEAMS; a piece of a slot has fewer than 2^31 words (of 16 bytes where every address,
  * stride and length allows it, else of 4 or 1). */
 typedef struct {

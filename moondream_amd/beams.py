@@ -89,7 +89,7 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, into: 
     """Slot b * beams + k of every state <- its slot b * beams + parents[b, k] (``parents``: int32 [batch, beams]), in place, or from ``states`` to ``into``
     (tensors of the same shapes and types that share no memory with them).  ``slot_dim``: the states' dimension of slots; the first batch * beams
     slots take part.  States may be views -- the rows of an answer in all layers' slabs, ``slab[:, :, :, first:last]`` -- whose dimensions
-    besides the slots' make at most two strides apart; no two of them share memory.  What lies in front of the answers is the same for all beams of an input and need not be moved."""
+    besides the slots' make at most two strides apart; no two of them share memory, nor does one that is written with another that is read.  What lies in front of the answers is the same for all beams of an input and need not be moved."""
     if parents.dim() != 2 or not 1 <= parents.shape[1] <= MAX_BEAMS or parents.shape[0] == 0:
         raise ValueError(f"parents {tuple(parents.shape)}: wanted [batch, 1 to {MAX_BEAMS} beams]")
     batch, beams = parents.shape

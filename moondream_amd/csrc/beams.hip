@@ -414,6 +414,8 @@ extern "C" md_status md_beam_select(const md_beam_args* a, void* stream) {
 extern "C" md_status md_state_reorder(const md_state_part* parts, int32_t n_parts, const int32_t* parents, int32_t batch, int32_t beams, void* stream) {
   MD_CHECK_ARG(parts && n_parts > 0 && parents && batch > 0 && batch <= 65535 && beams > 0 && beams <= MAXB);
   for (int i = 0; i < n_parts; ++i) MD_CHECK_ARG(part_ok(parts[i], (int64_t)batch * beams) && words_of(parts[i]) <= 0x7fffff00);
+  for (int i = 0; i < n_parts; ++i)  // (one launch moves many pieces: what one writes no other reads or writes)
+    for (int j = 0; j < n_parts; ++j) MD_CHECK_ARG(i == j || (parts[i].dst != parts[j].dst && parts[i].dst != parts[j].src));
   for (int done = 0; done < n_parts;) {
     Parts ps;
     ps.n = 0;

@@ -21,3 +21,11 @@ def test_a_vocabulary_that_32_bits_cannot_count_is_refused():
         assert (lib.md_beam_workspace_bytes(1, 2, vocab) > 0) == ok
         a = beam_args(batch=1, beams=2, vocab=vocab, ld=2**31, workspace=None)  # (a missing workspace: nothing is launched)
         assert lib.md_beam_select(C.byref(a), None) == (3 if ok else 1)
+
+
+def test_pieces_that_write_what_another_moves_are_refused():
+    lib, there = _lib.load(), 1 << 33
+    apart = dict(src=there, dst=there + AT)
+    for pieces in ([part(), part()], [part(src=AT, dst=AT), part(src=AT, dst=AT)], [part(), part(src=part().dst, dst=part().src)], [part(), part(**apart), part(src=part().dst, dst=2 * there)],
+                   [part(**apart), part(), part(src=2 * there, dst=part().dst)]):
+        assert lib.md_state_reorder((_lib.MdStatePart * len(pieces))(*pieces), len(pieces), AT, 2, 4, None) == 1

@@ -75,3 +75,18 @@ def test_states_between_one_another(beams):
     reorder_states([slab[:, 1]], parents.to(torch.int32).cuda(), into=[slab[:, 2]])
     reorder_states([slab[:, 0, :, 3:14]], parents.to(torch.int32).cuda(), into=[slab[:, 0, :, 30:41]])
     assert torch.equal(slab, want)
+
+
+def test_a_state_twice_and_two_states_in_each_others_place_are_refused():
+    from moondream_amd import _lib
+    from moondream_amd.beams import reorder_states
+
+    a, b = torch.arange(16.0, device="cuda").view(4, 4), torch.ones(4, 4, device="cuda")
+    parents = torch.tensor([[1, 0], [1, 1]], dtype=torch.int32, device="cuda")
+    for states, into in (([a, b, a], None), ([a, b], [b, a]), ([a, b], [torch.zeros_like(a)] * 2)):
+        with pytest.raises(_lib.MoondreamHipError):
+            reorder_states(states, parents, into=into)
+    assert torch.equal(a, torch.arange(16.0, device="cuda").view(4, 4)) and bool((b == 1).all())
+    both = [torch.zeros_like(a), torch.zeros_like(a)]
+    reorder_states([a, a], parents, into=both)  # one that is read twice is fine
+    assert torch.equal(both[0], a[[1, 0, 3, 3]]) and torch.equal(both[1], both[0])

@@ -204,21 +204,23 @@ __device__ __forceinline__ void softmax_block(f32x4 (&s)[NT][2], f16x8 (&pf)[NT]
         for (int i = 0; i < 4; ++i)
           if (key0 + t * 16 + 4 * q + i >= lim[ct]) s[ct][t][i] = -INFINITY;
   }
-  float top[NT];
+  float top[NT], shift[NT];  // (whether a weight is too large is asked in the units in which it is made: scores of 2^24 and more are whole numbers, sums with m and ev too)
   bool over = false;
 #pragma unroll
   for (int ct = 0; ct < NT; ++ct) {
     float a = s[ct][0][0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) a = fmaxf(a, s[ct][j >> 2][j & 3]);
-    top[ct] = __builtin_fmaf(a, ck, ev);
-    over |= top[ct] > m[ct] + SLACK;
+    top[ct] = a;
+    shift[ct] = ev - m[ct];
+    over |= __builtin_fmaf(a, ck, shift[ct]) > SLACK;
   }
   if (__any(over)) {
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) {
-      const float now = fmaxf(m[ct], over_q_max(top[ct]) - LIFT), f0 = __builtin_amdgcn_exp2f(m[ct] - now);
+      const float now = fmaxf(m[ct], over_q_max(__builtin_fmaf(top[ct], ck, ev)) - LIFT), f0 = __builtin_amdgcn_exp2f(m[ct] - now);
       m[ct] = now;
+      shift[ct] = ev - now;
       l[ct] *= f0;
 #pragma unroll
       for (int t = 0; t < VT; ++t) acc[ct][t] *= f0;
@@ -226,11 +228,10 @@ __device__ __forceinline__ void softmax_block(f32x4 (&s)[NT][2], f16x8 (&pf)[NT]
   }
 #pragma unroll
   for (int ct = 0; ct < NT; ++ct) {
-    const float shift = ev - m[ct];
     float sum = 0.f, e[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ct][j >> 2][j & 3], ck, shift));
+      e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ct][j >> 2][j & 3], ck, shift[ct]));
       sum += e[j];
     }
     l[ct] = __builtin_fmaf(sum, back, l[ct]);

@@ -107,3 +107,23 @@ def test_a_query_that_is_no_number_leaves_rows_alone_that_it_does_not_see(dim, t
     c.attention(well, ints([n]), weights=clean)
     seen = n - tokens + at + 1
     assert bool(torch.isnan(w[0, 0, :seen]).any()) and torch.equal(w[0, 0, seen:], clean[0, 0, seen:]) and torch.equal(w[0, 1], clean[0, 1])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch, tokens", [(1, 1), (40, 1), (2, 3), (2, 40), (20, 200)])
+def test_scores_of_millions_stay_finite(dim, batch, tokens):
+    """Scores of 2^24 and more in units of log2, which fp32 holds to whole numbers: outputs are still means of values."""
+    g = torch.Generator().manual_seed(dim + tokens)
+    n, heads = 4096, 32
+    k, v = torch.zeros(n, dim), torch.randn(n, dim, generator=g)
+    k[:, 0] = 4096.0
+    k[:, 1] = torch.arange(n) // U.BLOCK * 8.0  # block by block a little more, about as much as a running maximum may fall behind
+    c = one_slot(k.to(BF16), v.to(BF16), heads)
+    top = float(c.read(None, n)[1].abs().max())
+    q = torch.zeros(batch, tokens, heads, dim)
+    q[..., 0] = torch.randint(3000, 8192, (batch, tokens, heads), generator=g).float()
+    q[..., 1] = torch.rand(batch, tokens, heads, generator=g) * 2
+    got = c.attention(q.to(BF16).cuda(), ints([n] * batch), slot=ints([0] * batch), scale=1.0).float()
+    assert bool(torch.isfinite(got).all())
+    # fp16 weights are off by 2^-11, sums over keys by n * 2^-23, the output by 2^-8
+    assert float(got.abs().max()) <= top * (1 + 2.0**-11 + n * 2.0**-23) * (1 + 2.0**-8)

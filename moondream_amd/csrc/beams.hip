@@ -6,8 +6,8 @@
 //   part_kernel    one workgroup per (beam, piece of the vocabulary): the piece in registers; each wave's largest logits, its maximum and its sum
 //                  of exponentials
 //   choose_kernel  one workgroup per input, one wave per beam: sums joined in 64 bits, the pieces' lists merged, totals; then the beams' lists merged
-// Four beams of 51200 logits: 6.4 + 5.8 us, two launches' latency; 64 rows of 51200 bf16 logits 13.6 + 6.1 us; 64 rows of 131075 fp32 ones 27 us (1.2 TB/s: the
-// vector instructions, some 1700 for a wave's 2048 logits, 700 of them the sum's in 64 bits, follow the loads, as all workgroups run at once) and 13.9 us for 16 beams.
+// Four beams of 51200 logits: 6.4 + 5.8 us, two launches' latency; 64 rows of 51200 bf16 logits 13.3 + 6.0 us; 64 rows of 131075 fp32 ones 26 us (1.3 TB/s: the
+// vector instructions, some 1500 for a wave's 2048 logits, 600 of them the sum's in 64 bits, follow the loads, as all workgroups run at once) and 13.9 us for 16 beams.
 // States move at 6.8 TB/s (16 x 4 beams, 1.6 GB in 235 us).
 #include "layout.hpp"
 #include "wave_ops.hpp"
@@ -37,24 +37,24 @@ __device__ __forceinline__ float value_of(uint64_t c) {
 }
 __device__ __forceinline__ uint32_t index_of(uint64_t c) { return ~(uint32_t)c; }
 
-// exp(x), x <= 0, in 64 bits: 2^n e^r with |r| <= log(2) / 2, of which the series up to r^11 leaves 2^-47 (r^12 / 12!).  In fp32 two beams whose sums differ by
-// less than some 2^-24 would be ranked by rounding.  (64 rows of 131075 logits: 21.7 us with fp32's exponential.)
+// exp(x), x <= 0, in 64 bits: 2^n (1 + r q(r)), |r| <= log(2) / 2, q the polynomial of degree 8 through (e^r - 1) / r at nine Chebyshev points: 2^-44 off at most, and 1 at 0.
+// In fp32 two beams whose sums differ by less than some 2^-24 would be ranked by rounding.  (64 rows of 131075 logits: 25.8 us, 21.0 with fp32's exponential.)
 __device__ __forceinline__ double exp_of(double x) {
-  x = fmax(x, -750.);  // (e^-750 is 0)
-  const double n = rint(x * 1.4426950408889634), r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, x));  // (log(2) in two parts)
-  double p = 1. / 39916800;
-  p = fma(p, r, 1. / 3628800);
-  p = fma(p, r, 1. / 362880);
-  p = fma(p, r, 1. / 40320);
-  p = fma(p, r, 1. / 5040);
-  p = fma(p, r, 1. / 720);
-  p = fma(p, r, 1. / 120);
-  p = fma(p, r, 1. / 24);
-  p = fma(p, r, 1. / 6);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.);
-  p = fma(p, r, 1.);
-  return ldexp(p, (int)n);
+  constexpr double WHOLE = 6755399441055744.;  // 1.5 * 2^52: a sum with it ends in a whole number
+  x = fmax(x, -700.);  // (e^-700 beside 1 is nothing, and 2^n is no subnormal)
+  const double t = fma(x, 1.4426950408889634, WHOLE), n = t - WHOLE;
+  const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, x));  // (log(2) in two parts)
+  double q = 2.7625104515531025e-06;
+  q = fma(q, r, 2.4876166784942655e-05);
+  q = fma(q, r, 0.0001984120875246986);
+  q = fma(q, r, 0.0013888821672653597);
+  q = fma(q, r, 0.00833333335371942);
+  q = fma(q, r, 0.041666666890981904);
+  q = fma(q, r, 0.166666666666483);
+  q = fma(q, r, 0.49999999999797906);
+  q = fma(q, r, 1.0);
+  const uint64_t e = __builtin_bit_cast(uint64_t, fma(q, r, 1.));
+  return __builtin_bit_cast(double, e + (__builtin_bit_cast(uint64_t, t) << 52));  // (n into the exponent)
 }
 
 // 16 bytes of a row at any multiple of its elements' size

@@ -20,7 +20,7 @@
 // Few columns (decode): the waves of a workgroup share a column tile and take its blocks in turn, several workgroups share the keys, and a second
 // kernel joins their (O, m, l).  Bound by the cache's bytes: 64 x 1003 rows of 32 heads of 64 (198 MB) in 38 us, 5.2 TB/s, the rate of a large copy.
 // Many columns (prompts): every wave has its own columns, the converted operands come through LDS.  Bound by the sum of matrix and vector instructions, which
-// take turns on a SIMD where accumulators are in vector registers: 8 x 767 queries of 32 heads of 64 at 700 TFLOP/s (53 us; per block and wave 256 cycles of
+// take turns on a SIMD where accumulators are in vector registers: 8 x 767 queries of 32 heads of 64 at 700 TFLOP/s (53 us among other passes, 59 under the profiler; per block and wave 256 cycles of
 // products and 650 of softmax and conversion come to the time measured), 2 x 2048 queries of 32 on 8 heads of 128 over 6101 rows at 850 (280 us).
 // Accumulators in the other half of the registers, which overlap, were slower (68 and 345 us: inline assembly that the compiler does not schedule), as were
 // scores of the next block made beside the softmax of this one (63 and 302 us: registers).
@@ -444,7 +444,8 @@ __device__ __forceinline__ bool longest_first(const Params& p, int rank, int lan
 // Many columns: every wave has its own NT tiles, and the four waves share the conversion: of the next two blocks, waves 0 and 1 bring the keys, 2 and 3
 // the values into LDS as the products' operands (16 bytes per lane, one operand after another: no bank conflicts either way), while all work on
 // the two before.  32 columns per wave: 48 and 64 need the registers of a third wave per SIMD, and larger workgroups even out worse over the CUs
-// (8 x 767 queries, 32 heads of 64: 61 us against 66 and 67; 2 x 2048 queries over 6101 rows, 32 on 8 heads of 128: 359 against 364 and 559).
+// (compared before workgroups went by their reach, 8 x 767 queries, 32 heads of 64: 61 us against 66 and 67; 2 x 2048 queries over 6101 rows, 32 on 8 heads of 128: 359 against
+// 364 and 559.  The times now stand at the head of this file.)
 template <int HD, int NT>
 __global__ __launch_bounds__(256, 3) void prompt_kernel(Params p) {
   constexpr int VT = HD / 16, KF = 2 * (HD / 32), W = HD / 64;
@@ -686,8 +687,10 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
 }
 
 // The weight that every row got, from scores made again.  A wave holds 32 keys as operands (64 would leave registers for two waves per SIMD, and exponentials and
-// products of one wave follow each other: 201 us against 228 for 2 x 2048 queries over 6101 rows, 32 on 8 heads of 128); the columns that see them pass by, 64 at a time through LDS for the four waves.  Where that makes few workgroups the columns are shared out too (the first keys are
-// seen by all queries, the last by few: whole columns left 42 % of the CUs' time empty), and the shares added in their order afterwards.  The scores are the attention kernel's again (the same products in the same order), exp2(score - lse) is their softmax.
+// products of one wave follow each other: 201 us against 228 for 2 x 2048 queries over 6101 rows, 32 on 8 heads of 128); the columns that see them pass by, 64 at a time
+// through LDS for the four waves.  Where that makes few workgroups the columns are shared out too (the first keys are seen by all queries, the last by few: whole columns left
+// 42 % of the CUs' time empty), and the shares added in their order afterwards.  The scores are the attention kernel's again (the same products in the same order),
+// exp2(score - lse) is their softmax.
 template <int HD>
 __global__ __launch_bounds__(256, 4) void weights_kernel(Params p) {
   constexpr int KT = 2, QF = HD / 32, COLS = 64;  // key tiles, operands of a column tile, columns on their way

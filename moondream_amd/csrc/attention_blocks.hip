@@ -60,7 +60,8 @@ struct Params {
   float *scores;            // kept for the weights: [batch][kv_heads][cols][max_len to a whole block], in units of log2
   int score_rows, join_groups, batch, by_length, col_splits;
   float* wpart;             // of many columns shared out: [col_splits][batch][kv_heads][max_len to a whole block]
-  float *part, *part_ml, *lse, *weights;  // part: [batch][kv_heads][cols][splits][head_dim], part_ml: ... [splits][2], lse: [batch][kv_heads][cols]
+  float *part, *part_ml, *weights;  // part: [batch][kv_heads][cols][splits][head_dim], part_ml: ... [splits][2]
+  md_f32pair* norm;                 // with weights: [batch][kv_heads][cols], norm_of
 };
 
 // What a sequence has: its slot (-1: none), keys, queries, and the row of query 0
@@ -245,6 +246,13 @@ __device__ __forceinline__ void softmax_block(f32x4 (&s)[NT][2], f16x8 (&pf)[NT]
   }
 }
 
+// A column's maximum and the reciprocal of its sum (0, 0 where it sees no key): a row's weight is 2^(score - maximum) times that.  (A log of the sum taken from the score
+// instead rounds at its own size, and the hardware's log2 to one side: weights were 6e-7 too large.)  Where the sum is no number
+// the maximum says so alone, so that a weight of 0 stays 0.
+__device__ __forceinline__ md_f32pair norm_of(float m, float l) {
+  return l == 0.f ? md_f32pair{0.f, 0.f} : (l == l ? md_f32pair{m, 1.f / l} : md_f32pair{l, 1.f});
+}
+
 // Writes column `col`'s coordinates at0 .. of a split, or its output; o[n] unnormalised
 template <int HD, int N>
 __device__ __forceinline__ void store_column(const Params& p, int b, int kvh, int col, int split, int at0, const float (&o)[N], float m, float l, bool first) {
@@ -264,7 +272,7 @@ __device__ __forceinline__ void store_column(const Params& p, int b, int kvh, in
   bf16_t* out = p.o + (int64_t)b * p.o_bs + (int64_t)t * p.o_ts + (int64_t)(kvh * p.group + g) * p.o_hs + at0;
 #pragma unroll
   for (int i = 0; i < N; i += 4) *(u32x2*)(out + i) = u32x2{pack_bf16x2(o[i] * inv, o[i + 1] * inv), pack_bf16x2(o[i + 2] * inv, o[i + 3] * inv)};
-  if (p.lse && first) p.lse[c] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+  if (p.norm && first) p.norm[c] = norm_of(m, l);
 }
 
 // The columns of a wave: queries, how many keys each sees, and the most and the least of them (a later query never sees less)
@@ -645,25 +653,25 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
     bf16_t* out = p.o + (int64_t)b * p.o_bs + (int64_t)t * p.o_ts + (int64_t)(kvh * p.group + g) * p.o_hs + lane * N;
     if constexpr (N == 1) *out = f2bf(o[0] * inv);
     else *(uint32_t*)out = pack_bf16x2(o[0] * inv, o[1] * inv);
-    if (p.lse && lane == 0) p.lse[c0] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    if (p.norm && lane == 0) p.norm[c0] = norm_of(m, l);
     return;
   }
-  __shared__ float lse[24];  // (kept scores are those of up to 24 columns)
+  __shared__ md_f32pair norm[24];  // (kept scores are those of up to 24 columns)
   __shared__ int lims[24];
   const int first = (blockIdx.x - p.join_groups) * 1024;
   if (first >= sq.len) return;
   for (int col = wave; col < n_cols; col += 4) {
     const int64_t c0 = bh * p.cols + col;
-    float x;
+    md_f32pair x;
     if (p.splits > 1) {
       float m, l;
       join_factor(p.part_ml + c0 * p.splits * 2, p.splits, lane, m, l);
-      x = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+      x = norm_of(m, l);
     } else {
-      x = p.lse[c0];
+      x = p.norm[c0];
     }
     if (lane == 0) {
-      lse[col] = x;
+      norm[col] = x;
       lims[col] = limit_of(p, sq, sq.pos0 + query_of(p, col));
     }
   }
@@ -673,12 +681,12 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
   const float* sc = p.scores + bh * p.cols * p.score_rows + key;
   float w[4] = {};
   for (int col = 0; col < n_cols; ++col) {
-    const float ls = lse[col];
+    const md_f32pair of = norm[col];
     const int lim = lims[col];
     if (key >= lim) continue;  // (its scores may not be there)
     const f32x4 s = *(const f32x4*)(sc + (int64_t)col * p.score_rows);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] += key + i < lim ? __builtin_amdgcn_exp2f(s[i] - ls) : 0.f;
+    for (int i = 0; i < 4; ++i) w[i] += key + i < lim ? __builtin_amdgcn_exp2f(s[i] - of[0]) * of[1] : 0.f;
   }
   float* out = p.weights + ((int64_t)sq.slot * p.kv_heads + kvh) * p.ctx + key;
 #pragma unroll
@@ -690,12 +698,12 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
 // products of one wave follow each other: 201 us against 228 for 2 x 2048 queries over 6101 rows, 32 on 8 heads of 128); the columns that see them pass by, 64 at a time
 // through LDS for the four waves.  Where that makes few workgroups the columns are shared out too (the first keys are seen by all queries, the last by few: whole columns left
 // 42 % of the CUs' time empty), and the shares added in their order afterwards.  The scores are the attention kernel's again (the same products in the same order),
-// exp2(score - lse) is their softmax.
+// 2^(score - maximum) over the sum is their softmax.
 template <int HD>
 __global__ __launch_bounds__(256, 4) void weights_kernel(Params p) {
   constexpr int KT = 2, QF = HD / 32, COLS = 64;  // key tiles, operands of a column tile, columns on their way
   __shared__ u32x4 frag[2][COLS / 16 * QF][64];
-  __shared__ float lses[2][COLS];
+  __shared__ md_f32pair norms[2][COLS];
   __shared__ int lims[2][COLS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
   // (the first keys, which most queries see, first for all heads)
@@ -718,7 +726,7 @@ __global__ __launch_bounds__(256, 4) void weights_kernel(Params p) {
       a[t][2 * c + 1] = codes_bf16(x[2], x[3]);
     }
   }
-  const float* lse = p.lse + ((int64_t)b * p.kv_heads + kvh) * p.cols;
+  const md_f32pair* norm = p.norm + ((int64_t)b * p.kv_heads + kvh) * p.cols;
   const int n_cols = sq.rows * p.group;
   // queries from row wg_key0 on see something of these keys, those of the prefix if they begin within
   const int from = (wg_key0 < p.prefix ? 0 : min(max(wg_key0 - sq.pos0, 0), sq.rows)) * p.group;
@@ -727,7 +735,7 @@ __global__ __launch_bounds__(256, 4) void weights_kernel(Params p) {
 
   // wave w brings column tile w: every lane its 16-byte pieces of one column
   u32x4 st[QF];
-  float st_lse = INFINITY;
+  md_f32pair st_norm = {0.f, 0.f};
   int st_lim = 0;
   const bf16_t* queries = p.q + (int64_t)b * p.q_bs + (int64_t)(kvh * p.group) * p.q_hs + q * 16;
   const auto fetch = [&](int c0) {
@@ -735,14 +743,14 @@ __global__ __launch_bounds__(256, 4) void weights_kernel(Params p) {
     const bf16_t* at = queries + (int64_t)t * p.q_ts + (int64_t)g * p.q_hs;
 #pragma unroll
     for (int c = 0; c < QF; ++c) st[c] = *(const u32x4*)(at + (c >> 1) * 64 + (c & 1) * 8);
-    st_lse = lse[col];
+    st_norm = norm[col];
     st_lim = want < n_cols ? limit_of(p, sq, sq.pos0 + t) : 0;
   };
   const auto put = [&](int turn) {
 #pragma unroll
     for (int c = 0; c < QF; ++c) frag[turn][wave * QF + c][lane] = st[c] ^ u32x4{p.q_sign, p.q_sign, p.q_sign, p.q_sign};
     if (q == 0) {
-      lses[turn][wave * 16 + r] = st_lse;
+      norms[turn][wave * 16 + r] = st_norm;
       lims[turn][wave * 16 + r] = st_lim;
     }
   };
@@ -759,24 +767,27 @@ __global__ __launch_bounds__(256, 4) void weights_kernel(Params p) {
       }
 #pragma unroll
       for (int ct = 0; ct < COLS / 16; ++ct) {
-        const float ls = lses[turn][ct * 16 + r];
+        const md_f32pair of = norms[turn][ct * 16 + r];
         const int lim = lims[turn][ct * 16 + r];
         bf16x8 qf[1][QF];
 #pragma unroll
         for (int c = 0; c < QF; ++c) qf[0][c] = __builtin_bit_cast(bf16x8, frag[turn][ct * QF + c][lane]);
         f32x4 sc[1][KT], (&s)[KT] = sc[0];
         scores<HD, KT, 1>(a, qf, sc);
+        float top = of[0];
         if (__any(lim < key0 + 16 * KT)) {
+          const float none = top - top;  // 0, or no number: that is for the rows that the query sees, and for no other
+          top = none == none ? top : 0.f;
 #pragma unroll
           for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)  // (a sum that is no number stays out of rows that its query does not see)
-              w[t][j] += key0 + t * 16 + 4 * q + j < lim ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j], ck[t], -ls)) : 0.f;
-        } else {
+            for (int j = 0; j < 4; ++j) s[t][j] = key0 + t * 16 + 4 * q + j >= lim ? -INFINITY : s[t][j] + none;
+        }
 #pragma unroll
-          for (int t = 0; t < KT; ++t)
+        for (int t = 0; t < KT; ++t) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[t][j] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j], ck[t], -ls));
+          for (int j = 0; j < 4; ++j) w[t][j] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j], ck[t], -top)), of[1], w[t][j]);
+          asm volatile("" : "+v"(w[t][0]), "+v"(w[t][1]), "+v"(w[t][2]), "+v"(w[t][3]));  // (tile by tile: or the compiler begins more of them than there are registers for, 203 -> 267 us)
         }
       }
       __syncthreads();
@@ -829,7 +840,7 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(Params p) {
 struct Plan {
   bool decode, kept;  // kept: few columns' scores stay in the workspace for the weights
   int nt, waves, col_groups, splits, cols, score_rows, col_splits;
-  size_t part, ml, lse, scores, bytes;
+  size_t part, ml, norm, scores, bytes;
 };
 
 Plan plan_of(const md_kv8_cache* c, const md_kv8_attn_args* a) {
@@ -849,8 +860,8 @@ Plan plan_of(const md_kv8_cache* c, const md_kv8_attn_args* a) {
   const int64_t cols = (int64_t)a->batch * c->kv_heads * pl.cols;
   pl.part = 0;
   pl.ml = pl.splits > 1 ? cols * pl.splits * c->head_dim * 4 : 0;
-  pl.lse = pl.ml + (pl.splits > 1 ? cols * pl.splits * 2 * 4 : 0);
-  pl.scores = (pl.lse + (a->weights ? cols * 4 : 0) + 15) & ~(size_t)15;
+  pl.norm = pl.ml + (pl.splits > 1 ? cols * pl.splits * 2 * 4 : 0);
+  pl.scores = (pl.norm + (a->weights ? cols * 8 : 0) + 15) & ~(size_t)15;
   pl.score_rows = blocks * BLK;
   const int64_t key_groups = (int64_t)((max_len + 127) / 128) * c->kv_heads * a->batch;
   pl.col_splits = (int)std::max<int64_t>(1, std::min<int64_t>({(3000 + key_groups - 1) / key_groups, (pl.cols + 255) / 256, 16}));
@@ -919,7 +930,7 @@ extern "C" md_status md_kv8_attention(const md_kv8_cache* cache, const md_kv8_at
   char* ws = (char*)a->workspace;
   p.part = (float*)(ws + pl.part);
   p.part_ml = (float*)(ws + pl.ml);
-  p.lse = a->weights ? (float*)(ws + pl.lse) : nullptr;
+  p.norm = a->weights ? (md_f32pair*)(ws + pl.norm) : nullptr;
   p.weights = a->weights;
   p.scores = pl.kept ? (float*)(ws + pl.scores) : nullptr;
   p.score_rows = pl.score_rows;

@@ -18,3 +18,20 @@ def test_weights_from_kept_scores_and_from_keys_again(dim, group, tokens, batch,
     attend(c, k, v, q, lens, weights=True, decay=0.0, q_rows=[tokens // 2 + 1, 0, tokens, 1, tokens][:batch], prefix=50, max_len=length - 5)
     c, k, v = filled(g, batch, length, kv_heads, dim)  # (here every row of every slot may be seen)
     attend(c, k, v, q, lens, weights=True, slot=[(i + 1) % (batch + 1) for i in range(batch)], q_pos0=[3 * i - 1 for i in range(batch)])  # the last slot there is not
+
+
+@pytest.mark.parametrize("dim, group, tokens, n", [(64, 4, 1, 9000), (128, 8, 1, 30000), (128, 4, 8, 9000), (64, 1, 200, 3000), (128, 2, 300, 4000)])
+def test_weights_lean_to_no_side(dim, group, tokens, n):
+    """Roundings are to the nearest; what may lean is the hardware's exponential (an ulp, 2^-23) against the sum's own, and the sum's reciprocal (2^-24): less than 2^-22 together.
+    The scores' own roundings have either sign: over all rows and heads their mean is less than a quarter of that."""
+    import blocks_util as U
+
+    g = torch.Generator().manual_seed(n)
+    heads = 4
+    c, k, v = filled(g, 1, n, heads, dim)
+    q = (torch.randn(1, tokens, heads * group, dim, generator=g) * 0.7).to(torch.bfloat16)
+    w = torch.zeros(1, heads, c.ctx, device="cuda")
+    c.attention(q.cuda(), torch.tensor([n], dtype=torch.int32, device="cuda"), weights=w, decay=0.0)
+    _, want, _, _, _ = U.attention(q[0], k[0], v[0], n, n - tokens, 0, dim**-0.5)
+    off = (w[0, :, :n].cpu().double() / want[:, :n] - 1)[want[:, :n] > 1e-20]
+    assert abs(float(off.mean())) < 2.0**-22, float(off.mean())

@@ -695,7 +695,7 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
 }
 
 // The weight that every row got, from scores made again.  A wave holds 32 keys as operands (64 would leave registers for two waves per SIMD, and exponentials and
-// products of one wave follow each other: 201 us against 228 for 2 x 2048 queries over 6101 rows, 32 on 8 heads of 128); the columns that see them pass by, 64 at a time
+// products of one wave follow each other: 201 us against 228 at that step for 2 x 2048 queries over 6101 rows, 32 on 8 heads of 128); the columns that see them pass by, 64 at a time
 // through LDS for the four waves.  Where that makes few workgroups the columns are shared out too (the first keys are seen by all queries, the last by few: whole columns left
 // 42 % of the CUs' time empty), and the shares added in their order afterwards.  The scores are the attention kernel's again (the same products in the same order),
 // 2^(score - maximum) over the sum is their softmax.

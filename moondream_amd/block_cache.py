@@ -165,7 +165,7 @@ class BlockCache:
             if out.shape != q.shape:
                 raise ValueError(f"out: {tuple(out.shape)}, wanted {tuple(q.shape)}")
             os = self._rows_of(out, "out")
-            if 0 in os:  # (an expanded dimension: outputs would be written over one another)
+            if any(s == 0 and n > 1 for s, n in zip(os, q.shape)):  # (an expanded dimension: outputs would be written over one another)
                 raise ValueError(f"out: strides {os}")
         if tokens == 0:
             return out

@@ -35,3 +35,14 @@ def test_weights_lean_to_no_side(dim, group, tokens, n):
     _, want, _, _, _ = U.attention(q[0], k[0], v[0], n, n - tokens, 0, dim**-0.5)
     off = (w[0, :, :n].cpu().double() / want[:, :n] - 1)[want[:, :n] > 1e-20]
     assert abs(float(off.mean())) < 2.0**-22, float(off.mean())
+
+
+def test_an_output_of_one_sequence_or_token_may_have_any_stride_there():
+    g = torch.Generator().manual_seed(3)
+    c, _, _ = filled(g, 1, 64, 2, 64)
+    q = torch.randn(1, 1, 4, 64, generator=g).to(torch.bfloat16).cuda()
+    n = torch.tensor([60], dtype=torch.int32, device="cuda")
+    out = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda").as_strided((1, 1, 4, 64), (0, 0, 64, 1))
+    assert torch.equal(c.attention(q, n, out=out), c.attention(q, n))
+    with pytest.raises(ValueError):
+        c.attention(q, n, out=out[:, :, :1].expand(1, 1, 4, 64))
